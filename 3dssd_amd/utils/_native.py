@@ -50,6 +50,15 @@ SIGNATURES = {
     "sa_group_mlp_plan": [_c_int] * 3 + [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp],
     "sa_group_mlp_plan2": [_c_int] * 3 + [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp],
     "sa_dense": [_c_long, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _vp],
+    "sa_dense_forward_ws": [_c_int, _c_long, _c_int, _c_int, _c_int, _vp],
+    "sa_dense_forward": [_c_int, _c_long, _c_int, _c_int, _vp, _c_long, _vp, _c_long, _vp, _c_int, _vp, _c_long, _c_int, _vp, _vp,
+                         _vp, ctypes.c_ulong, _vp],
+    "sa_dense_backward_ws": [_c_int, _c_long] + [_c_int] * 5 + [_vp],
+    "sa_dense_backward": [_c_int, _c_long, _c_int, _c_int] + [_vp, _c_long] * 4 + [_c_int, _vp, _vp, _vp, _c_int, _vp,
+                          ctypes.c_ulong, _vp],
+    "sa_global_norm_ws": [_c_int, _vp],
+    "sa_global_norm": [_c_int, _vp, _vp, _vp, _vp, _vp, ctypes.c_ulong, _vp],
+    "sa_clip_by_global_norm": [_c_int, _vp, _vp, _vp, _vp, _c_float, _vp, _vp, _vp, ctypes.c_ulong, _vp],
     "sa_decode_anchor_free": [_c_int] * 4 + [_vp] * 7,
     "sa_boxes_to_bev": [_c_long, _vp, _vp, _vp],
     "sa_nms_bev": [_c_int] * 4 + [_c_float, _vp, _vp, _vp, _vp, _vp],

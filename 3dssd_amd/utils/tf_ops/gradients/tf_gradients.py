@@ -1,0 +1,143 @@
+"""The global norm of a list of gradients and clipping by it, on torch-ROCm tensors, backed by csrc/gradnorm.hip through the
+C ABI of include/sa_ops.h.
+
+The reference's training graph clips every tower's gradients to a global norm of 5 (lib/core/trainer.py:120-155); the names,
+the argument order and the results follow the TensorFlow functions it calls.  The gradients may be of different types
+(float32, bfloat16, float16); None entries are passed over.
+"""
+import bisect
+import ctypes
+
+import torch
+
+from .. import _tensor as T
+from ... import _native as N
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check(t, name):
+    T.require(isinstance(t, torch.Tensor), "%s must be a torch.Tensor" % name)
+    T.require(t.is_cuda, "%s must live on the GPU (the HIP path has no CPU fallback)" % name)
+    T._on_current_device(t, name)
+    T.require(t.dtype in TYPES, "%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+
+
+def _dense_memory(t):
+    """Every element of one block of memory exactly once, in any order of dimensions (a transposed matrix passes)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _arrays(ts):
+    k = len(ts)
+    return ((ctypes.c_void_p * k)(*[t.data_ptr() for t in ts]), (ctypes.c_long * k)(*[t.numel() for t in ts]),
+            (ctypes.c_int * k)(*[TYPES[t.dtype] for t in ts]))
+
+
+def _gather(t_list, op):
+    T.require(isinstance(t_list, (list, tuple)), "%s expects a list of tensors" % op)
+    ts = []
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for i, t in enumerate(t_list):
+        if t is None:
+            continue
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device and t.dtype in TYPES):
+            _check(t, "t_list[%d]" % i)
+        ts.append(t)
+    return ts
+
+
+def _scratch(count):
+    n = ctypes.c_ulong()
+    N.check(N.lib().sa_global_norm_ws(count, ctypes.byref(n)), "global_norm")
+    return torch.empty(n.value, dtype=torch.uint8, device="cuda"), n.value
+
+
+def global_norm(t_list):
+    """sqrt of the sum of all squares, a float32 scalar tensor on the GPU.  Sums are held in 64 bits, in a fixed order."""
+    ts = [t if _dense_memory(t) else t.contiguous() for t in _gather(t_list, "GlobalNorm")]
+    T.require(torch.cuda.is_available(), "GlobalNorm needs a GPU (the HIP path has no CPU fallback)")
+    norm = torch.empty((), dtype=torch.float32, device="cuda")
+    p, n, kinds = _arrays(ts)
+    ws, size = _scratch(len(ts))
+    N.check(N.lib().sa_global_norm(len(ts), p, n, kinds, norm.data_ptr(), ws.data_ptr(), size, N.current_stream()), "global_norm")
+    return norm
+
+
+def _overlap(ts):
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
+    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+
+def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
+    """([t * clip_norm / max(norm, clip_norm) for t in t_list], norm).
+
+    clip_norm: a positive number.  use_norm: a float32 scalar tensor on the GPU to use in place of the list's own norm (of
+    gradients spread over several processes, say).  A norm that is NaN or infinite makes every result NaN, as in
+    TensorFlow.  None entries stay None.
+
+    out: None for new tensors, t_list itself to clip in place (nothing is written where the norm is within bounds), or a
+    list of tensors of the same shapes and types.  Results must not overlap one another, nor any gradient but their own,
+    which they may only share whole; each must be dense in memory, in its gradient's order of dimensions."""
+    ts = _gather(t_list, "ClipByGlobalNorm")
+    clip = float(clip_norm)
+    T.require(clip > 0, "ClipByGlobalNorm expects a positive clip_norm")
+    T.require(torch.cuda.is_available(), "ClipByGlobalNorm needs a GPU (the HIP path has no CPU fallback)")
+    if use_norm is not None:
+        _check(use_norm, "use_norm")
+        T.require(use_norm.dtype == torch.float32 and use_norm.numel() == 1, "ClipByGlobalNorm expects a float32 scalar use_norm")
+    if out is None:
+        ts = [t if _dense_memory(t) else t.contiguous() for t in ts]
+        results = [torch.empty_like(t) for t in ts]
+        given = None
+    else:
+        T.require(isinstance(out, (list, tuple)) and len(out) == len(t_list), "ClipByGlobalNorm expects as many out tensors as gradients")
+        in_place = out is t_list
+        given = [o for o, t in zip(out, t_list) if t is not None]
+        results = given
+        for i, (t, o) in enumerate(zip(ts, results)):
+            if not in_place:
+                _check(o, "out[%d]" % i)
+                T.require(o.shape == t.shape and o.dtype == t.dtype, "out[%d] differs from its gradient in shape or type" % i)
+                T.require(t.numel() < 2 or all(a == b for a, b, n in zip(o.stride(), t.stride(), t.shape) if n != 1),
+                          "out[%d] differs from its gradient in strides" % i)
+            T.require(_dense_memory(t), "gradient %d is not dense in memory: it cannot be clipped into out" % i)
+        T.require(not _overlap(results), "ClipByGlobalNorm cannot write tensors that overlap")
+        moved = [] if in_place else [t for t, o in zip(ts, results) if t.data_ptr() != o.data_ptr()]
+        T.require(not _overlap_between(results, moved), "ClipByGlobalNorm cannot write over another gradient")
+        T.require(use_norm is None or not _overlap_between(results, [use_norm]), "ClipByGlobalNorm cannot write over use_norm")
+    k = len(ts)
+    p, n, kinds = _arrays(ts)
+    o = (ctypes.c_void_p * k)(*[t.data_ptr() for t in results])
+    if use_norm is None:
+        norm = torch.empty((), dtype=torch.float32, device="cuda")
+        ws, size = _scratch(k)
+        N.check(N.lib().sa_clip_by_global_norm(k, p, o, n, kinds, clip, None, norm.data_ptr(), ws.data_ptr(), size,
+                                               N.current_stream()), "clip_by_global_norm")
+    else:
+        norm = use_norm
+        N.check(N.lib().sa_clip_by_global_norm(k, p, o, n, kinds, clip, norm.data_ptr(), None, None, 0, N.current_stream()),
+                "clip_by_global_norm")
+    it = iter(results)
+    return [None if t is None else next(it) for t in t_list], norm
+
+
+def _overlap_between(written, read):
+    """Does any tensor of `written` share bytes with one of `read`?  (`written` do not overlap one another.)"""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written if t.numel())
+    starts = [s[0] for s in spans]
+    for t in read:
+        if not t.numel():
+            continue
+        lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+        i = bisect.bisect_left(starts, hi) - 1       # the last written span that starts before this one ends
+        if i >= 0 and spans[i][1] > lo:
+            return True
+    return False

@@ -250,6 +250,37 @@ int sa_group_mlp_max_layer(int nscale, int b, int n, int m, const int *ns, int c
 int sa_dense(long rows, int K, int N, const float *x, const void *wpack, const float *bias, int relu,
              float *y, sa_stream_t stream);
 
+/* ---- the dense layer on plain weights, its gradient, and gradient clipping (training, serving) ------------------------- */
+
+/* y = act(x W + bias) + res.  dtype: 0 fp32, 1 bf16, 2 fp16, of x [rows,cin] (ldx elements between rows), W [cin,cout]
+ * (ldw), res [rows,cout] (ldr; nullable), y and pre [rows,cout] (dense; pre = x W + bias, nullable); bias [cout] (nullable)
+ * is fp32 where bias_f32 is set, else of that type.  act: 0 none, 1 ReLU, 2 GELU (normal integral), 3 GELU (tanh form),
+ * 4 SiLU.  Any sizes, strides and alignments of whole elements; sums in fp32, one rounding per output, no atomics: the
+ * same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has 16-byte aligned base and
+ * rows), 16-byte aligned, used until the call's work on the stream is done. */
+int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes);
+int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
+                     const void *bias, int bias_f32, const void *res, long ldr, int act, void *y, void *pre, void *ws,
+                     unsigned long ws_bytes, sa_stream_t stream);
+/* Gradient: dz = g act'(z), dx = dz W^T [rows,cin], dw = x^T dz [cin,cout], db = column sums of dz [cout] (fp32 where
+ * db_f32), each nullable and dense; g, z [rows,cout] (ldg, ldz; z = pre of the forward call, unused with act 0).  16-bit
+ * types round dz once, as an operand of the products.  want (of the _ws call): bit 0 / 1 / 2 = dx / dw / db; flags: bit
+ * 0 / 1 / 2 = x / W / g has 16-byte aligned base and rows. */
+int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes);
+int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
+                      const void *g, long ldg, const void *z, long ldz, int act, void *dx, void *dw, void *db, int db_f32,
+                      void *ws, unsigned long ws_bytes, sa_stream_t stream);
+/* tf.global_norm / tf.clip_by_global_norm as lib/core/trainer.py:120-155 applies them: norm = sqrt(sum of squares) (64-bit
+ * sums, one fp32 scalar on the device), out[i] = p[i] * clip / max(norm, clip); a norm that is not finite makes every
+ * output NaN.  p, out, n (elements), type (as above): HOST arrays of `count` entries, read before the call returns.
+ * out[i] == p[i] clips in place; no other overlap.  use_norm (device, nullable) replaces the list's own norm: norm and ws
+ * are then unused. */
+int sa_global_norm_ws(int count, unsigned long *bytes);
+int sa_global_norm(int count, const void *const *p, const long *n, const int *type, float *norm, void *ws,
+                   unsigned long ws_bytes, sa_stream_t stream);
+int sa_clip_by_global_norm(int count, const void *const *p, void *const *out, const long *n, const int *type, float clip,
+                           const float *use_norm, float *norm, void *ws, unsigned long ws_bytes, sa_stream_t stream);
+
 /* vote_layer tail (layers_util.py:21-23): out = xyz + clip(off, lo, -lo), lo = MAX_TRANSLATE_RANGE. */
 int sa_vote_translate(long npoints, const float *xyz, const float *off, float lo_x, float lo_y,
                       float lo_z, float *out, sa_stream_t stream);

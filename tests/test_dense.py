@@ -1,0 +1,453 @@
+"""tf_ops/dense: the dense layer with its epilogue, and its gradient, against the formulas in 64 bits.
+
+Bounds, per element.  u = 2^-24 is half a step of fp32, h = eps / 2 half a step of the layer's type.  A sum of K products
+computed in fp32 in any order is off by about sqrt(K) u times S = sum |x||w| (rounding errors of random sign; 8 sqrt(K) is
+eight standard deviations), plus a few u for what happens to the sum afterwards: bias, activation (Lipschitz constant < 1.2,
+exp and erfc within a few u of values no larger than |z| + 1), residual.  The result is rounded once: h |y|.  In the
+gradient the 16-bit types round dz once (h |dz| per factor), which passes through the products with |w| and |x|."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from conftest import pkg
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
+
+
+def _mod():
+    return pkg("utils.tf_ops.dense.tf_dense")
+
+
+def _half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def _tiny(dt):
+    return torch.finfo(dt).smallest_normal * torch.finfo(dt).eps       # half steps below the normal range
+
+
+def _act64(z, act):
+    if act is None:
+        return z
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "gelu":
+        return z * torch.special.ndtr(z)
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z * torch.sigmoid(z)
+
+
+def _slope64(z, act):
+    if act is None:
+        return torch.ones_like(z)
+    if act == "relu":
+        return (z > 0).double()
+    if act == "gelu":
+        return torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "gelu_tanh":
+        t = torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+        return 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z ** 2)
+    s = torch.sigmoid(z)
+    return s * (1 + z * (1 - s))
+
+
+def _sum_bound(k):
+    return (8 * math.sqrt(max(k, 1)) + 16) * U
+
+
+def _within(got, want, bound, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bool(bad.any()), "%s: %d of %d outside, worst %.3g of its bound at %s" % (
+        what, int(bad.sum()), bad.numel(), float((err / bound).max()), bad.nonzero()[0].tolist())
+
+
+def _check_forward(x, w, b, act, res, out, pre):
+    dt = x.dtype
+    xd, wd = x.double(), w.double()
+    z = xd @ wd.contiguous()
+    s = xd.abs() @ wd.abs().contiguous()
+    if b is not None:
+        z, s = z + b.double(), s + b.double().abs()
+    dz = _sum_bound(w.shape[0]) * s + 4 * U * z.abs()
+    if pre is not None:
+        _within(pre, z, _half(dt) * (z.abs() + dz) + dz + _tiny(dt), "preact")
+    y = _act64(z, act)
+    bound = 1.2 * dz + 16 * U * (z.abs() + 1) * (act not in (None, "relu"))
+    if res is not None:
+        y = y + res.double()
+        bound = bound + 2 * U * (y.abs() + res.double().abs())
+    _within(out, y, _half(dt) * (y.abs() + bound) + bound + _tiny(dt), "out")
+
+
+def _check_grad(x, w, g, act, z, dx, dw, db):
+    dt = x.dtype
+    gd = g.double()
+    d = gd if act is None else gd * _slope64(z.double(), act)
+    # slope: a few steps of terms no larger than 1.2 (1 + |z|); one rounding to the type where there is an activation
+    dd = 0 * d if act is None else 32 * U * gd.abs() * (1 + z.double().abs()) + _tiny(torch.float32)
+    dr = dd if act is None or dt == torch.float32 else dd + _half(dt) * (d.abs() + dd) + _tiny(dt)
+    xd, wd = x.double(), w.double()
+    if dx is not None:
+        want = d @ wd.t().contiguous()
+        b = (_sum_bound(w.shape[1]) * (d.abs() + dr) + dr) @ wd.abs().t().contiguous()
+        _within(dx, want, _half(dt) * (want.abs() + b) + b + _tiny(dt), "grad_inputs")
+    if dw is not None:
+        xt = xd.t().contiguous()
+        want = xt @ d
+        b = xt.abs() @ (_sum_bound(x.shape[0]) * (d.abs() + dr) + dr)
+        _within(dw, want, _half(dt) * (want.abs() + b) + b + _tiny(dt), "grad_weights")
+    if db is not None:
+        want = d.sum(0)
+        b = (_sum_bound(x.shape[0]) * (d.abs() + dd) + dd).sum(0)
+        _within(db, want, _half(db.dtype) * (want.abs() + b) + b + _tiny(db.dtype), "grad_biases")
+
+
+def _rand(gpu, shape, dt, seed, scale=1.0):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=gpu) * scale).to(dt)
+
+
+# (rows, cin, cout): one row to thousands, odd and aligned widths, one column, one channel, tiles' edges and one past them
+SIZES = [(1, 1, 1), (1, 64, 8), (1, 1027, 515), (3, 5, 7), (17, 67, 33), (64, 64, 64), (65, 65, 65), (128, 256, 128),
+         (129, 257, 130), (300, 131, 1), (5, 2048, 24), (33, 4096, 257), (1000, 96, 200), (257, 512, 384), (515, 771, 259),
+         (2048, 512, 128), (1, 4096, 1024), (8, 1024, 1000), (16, 640, 512), (31, 1000, 2048), (4099, 40, 72)]
+
+
+# ------------------------------------------------------------------------------------------------------- CPU: refusals
+def test_cpu_tensors_and_unknown_activations_are_refused():
+    m = _mod()
+    x, w = torch.zeros(2, 3), torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        m.dense(x, w)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        m.dense_grad(x, w, torch.zeros(2, 4))
+    with pytest.raises(ValueError, match="torch.Tensor"):
+        m.dense(None, w)
+
+
+def test_the_c_entries_refuse_what_they_cannot_compute():
+    lib = pkg("utils._native").lib()
+    n = ctypes.c_ulong()
+    by = ctypes.byref(n)
+    assert lib.sa_dense_forward_ws(3, 1, 1, 1, 0, by) == -1 and lib.sa_dense_forward_ws(0, -1, 1, 1, 0, by) == -1
+    assert lib.sa_dense_forward_ws(0, 1, 1, 1, 0, None) == -1
+    assert lib.sa_dense_backward_ws(0, 1, 1, 1, 9, 7, 0, by) == -1 and lib.sa_dense_backward_ws(0, 1, 1, 1, 0, 8, 0, by) == -1
+    p = 1 << 20                                        # an address that is never dereferenced: every call below is refused
+    fwd = lambda **k: lib.sa_dense_forward(*[k.get(a, d) for a, d in (   # noqa: E731
+        ("dtype", 1), ("rows", 4), ("cin", 8), ("cout", 8), ("x", p), ("ldx", 8), ("w", p), ("ldw", 8), ("bias", None), ("bf", 0),
+        ("res", None), ("ldr", 0), ("act", 0), ("y", p), ("pre", None), ("ws", None), ("wsb", 0), ("stream", None))])
+    assert fwd(dtype=7) == -1 and fwd(act=5) == -1 and fwd(act=-1) == -1 and fwd(rows=-1) == -1
+    assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
+    assert fwd(ldx=7) == -1 and fwd(ldw=7) == -1 and fwd(res=p, ldr=7) == -1
+    assert fwd(rows=0) == 0 and fwd(cout=0) == 0       # nothing to compute
+    assert lib.sa_dense_forward_ws(1, 4, 4096, 8, 3, by) == 0 and n.value > 0
+    assert fwd(cin=4096, ldx=4096) == -1               # scratch missing
+    assert fwd(cin=4096, ldx=4096, ws=p, wsb=n.value - 1) == -1
+    bwd = lambda **k: lib.sa_dense_backward(*[k.get(a, d) for a, d in (   # noqa: E731
+        ("dtype", 1), ("rows", 4), ("cin", 8), ("cout", 8), ("x", p), ("ldx", 8), ("w", p), ("ldw", 8), ("g", p), ("ldg", 8),
+        ("z", p), ("ldz", 8), ("act", 1), ("dx", p), ("dw", p), ("db", p), ("df", 0), ("ws", None), ("wsb", 0), ("stream", None))])
+    assert bwd() == -1                                 # scratch missing
+    assert bwd(g=None) == -1 and bwd(z=None) == -1 and bwd(x=None) == -1 and bwd(w=None) == -1 and bwd(ldg=7) == -1
+    assert bwd(dx=None, dw=None, db=None) == 0
+
+
+# --------------------------------------------------------------------------------------------------------- GPU: values
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_dense_matches_64_bits(gpu, size, dt):
+    m = _mod()
+    rows, cin, cout = size
+    i = SIZES.index(size)
+    x, w = _rand(gpu, (rows, cin), dt, i), _rand(gpu, (cin, cout), dt, 100 + i, math.sqrt(2.0 / cin))
+    b = _rand(gpu, (cout,), torch.float32 if i % 2 else dt, 200 + i)
+    res = _rand(gpu, (rows, cout), dt, 300 + i)
+    act = ACTS[i % 5]
+    out, pre = m.dense(x, w, b, activation=act, residual=res, return_preact=True)
+    assert out.dtype == dt and out.shape == (rows, cout) and pre.shape == out.shape
+    _check_forward(x, w, b, act, res, out, pre)
+    plain = m.dense(x, w)
+    _check_forward(x, w, None, None, None, plain, None)
+    assert torch.equal(m.dense(x, w), plain)           # the same call, the same bits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_every_activation_over_its_whole_range(gpu, act, dt):
+    # one channel in, weight 1: z is the input itself, from the tails to zero
+    m = _mod()
+    x = torch.cat([torch.linspace(-40, 40, 4001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e4, -1e4])]).to(gpu).to(dt)[:, None]
+    w = torch.ones(1, 1, dtype=dt, device=gpu)
+    out, pre = m.dense(x, w, activation=act, return_preact=True)
+    assert torch.equal(pre, x + 0)
+    _check_forward(x, w, None, act, None, out, pre)
+    g = torch.ones_like(x)
+    dx, dw, db = m.dense_grad(x, w, g, biases=torch.zeros(1, dtype=dt, device=gpu), activation=act, preact=pre)
+    _check_grad(x, w, g, act, pre, dx, dw, None)       # (4 007 terms of which all but a few are small: see the sums' test)
+    assert torch.isfinite(out).all() and torch.isfinite(dx).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_dense_grad_matches_64_bits(gpu, size, dt):
+    m = _mod()
+    rows, cin, cout = size
+    i = SIZES.index(size)
+    act = ACTS[(i + 2) % 5]
+    x, w = _rand(gpu, (rows, cin), dt, i), _rand(gpu, (cin, cout), dt, 100 + i, math.sqrt(2.0 / cin))
+    g, z = _rand(gpu, (rows, cout), dt, 200 + i, 0.05), _rand(gpu, (rows, cout), dt, 300 + i)
+    b = torch.empty(cout, dtype=torch.float32 if i % 2 else dt, device=gpu)
+    dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z)
+    assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape and db.dtype == b.dtype
+    _check_grad(x, w, g, act, z, dx, dw, db)
+    only_x = m.dense_grad(x, w, g, activation=act, preact=z, needs=(True, False))
+    only_w = m.dense_grad(x, w, g, activation=act, preact=z, needs=(False, True))
+    assert only_x[1] is None and only_x[2] is None and torch.equal(only_x[0], dx)
+    assert only_w[0] is None and torch.equal(only_w[1], dw)
+
+
+@pytest.mark.gpu
+def test_dense_grad_against_differences(gpu):
+    # phi(t) = <g, dense(x + t dx, w + t dw, b + t db)> has the slope that the gradients give; central differences in fp32:
+    # error h^2 / 6 phi''' ~ 1e-4 of the terms' size plus the rounding of phi, u |phi| / h ~ 1e-4
+    m = _mod()
+    rows, cin, cout = 37, 61, 45
+    for k, act in enumerate(["gelu", "gelu_tanh", "silu", None]):
+        x, w, b = _rand(gpu, (rows, cin), torch.float32, k), _rand(gpu, (cin, cout), torch.float32, 10 + k, 0.15), _rand(
+            gpu, (cout,), torch.float32, 20 + k)
+        g = _rand(gpu, (rows, cout), torch.float32, 30 + k)
+        vx, vw, vb = (_rand(gpu, t.shape, torch.float32, 40 + k + i, 0.1) for i, t in enumerate((x, w, b)))
+        h = 1e-2
+        phi = [float((m.dense(x + s * h * vx, w + s * h * vw, b + s * h * vb, activation=act).double() * g.double()).sum())
+               for s in (1, -1)]
+        _, z = m.dense(x, w, b, activation=act, return_preact=True)
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z)
+        slope = sum(float((a.double() * v.double()).sum()) for a, v in ((dx, vx), (dw, vw), (db, vb)))
+        size = math.sqrt(sum(float((a.double() * v.double()).pow(2).sum()) for a, v in ((dx, vx), (dw, vw), (db, vb))))
+        assert abs((phi[0] - phi[1]) / (2 * h) - slope) < 2e-3 * max(size, abs(slope)), act
+
+
+# ---------------------------------------------------------------------------------------- GPU: layouts, edges, neighbours
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_strides_offsets_and_leading_dimensions(gpu, dt):
+    m = _mod()
+    nan = float("nan")
+    for cin, cout, pad in ((64, 72, 8), (67, 33, 5), (512, 256, 64), (131, 515, 1)):
+        rows = 150
+        big_x, big_w = torch.full((rows, cin + pad), nan, dtype=dt, device=gpu), torch.full((cin, cout + pad), nan, dtype=dt, device=gpu)
+        big_r, big_g = (torch.full((rows, cout + pad), nan, dtype=dt, device=gpu) for _ in range(2))
+        x, w, r, g = big_x[:, pad:], big_w[:, :cout], big_r[:, pad:], big_g[:, :cout]     # NaN between the rows
+        x.copy_(_rand(gpu, x.shape, dt, 1)); w.copy_(_rand(gpu, w.shape, dt, 2, 0.1))     # noqa: E702
+        r.copy_(_rand(gpu, r.shape, dt, 3)); g.copy_(_rand(gpu, g.shape, dt, 4))          # noqa: E702
+        b = _rand(gpu, (2 * cout,), dt, 5)[::2]                                           # a strided bias
+        out, pre = m.dense(x, w, b, activation="silu", residual=r, return_preact=True)
+        _check_forward(x, w, b, "silu", r, out, pre)
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation="silu", preact=pre)
+        _check_grad(x, w, g, "silu", pre, dx, dw, db)
+        # a transposed weight, a column-major input, broadcast rows and residual
+        wt = w.t().contiguous().t()
+        xt = x.t().contiguous().t()
+        assert not wt.is_contiguous() and not xt.is_contiguous()
+        ref = m.dense(x.contiguous(), w.contiguous(), activation="relu")
+        assert torch.equal(m.dense(xt, wt, activation="relu"), ref)
+        one = x[:1].expand(rows, cin)
+        _check_forward(one, w, None, None, r[:1].expand(rows, cout), m.dense(one, w, residual=r[:1].expand(rows, cout)), None)
+        # more leading dimensions, and none
+        x3 = x.contiguous().view(3, 50, cin)
+        assert torch.equal(m.dense(x3, w.contiguous(), activation="relu"), ref.view(3, 50, cout))
+        assert m.dense(x3[:, ::2], w).shape == (3, 25, cout)
+        _check_forward(x3[:, ::2].reshape(-1, cin), w, None, None, None, m.dense(x3[:, ::2], w).view(-1, cout), None)
+        v = m.dense(x[0], w)
+        assert v.shape == (cout,)
+        _check_forward(x[:1], w, None, None, None, v[None], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_empty_sizes(gpu, dt):
+    m = _mod()
+    new = lambda *s: torch.randn(*s, device=gpu).to(dt)  # noqa: E731
+    assert m.dense(new(0, 5), new(5, 7)).shape == (0, 7) and m.dense(new(3, 5), new(5, 0)).shape == (3, 0)
+    b, r = new(7), new(3, 7)
+    out = m.dense(new(3, 0), new(0, 7), b, activation="relu", residual=r)
+    assert torch.equal(out, (torch.relu(b.float()) + r.float()).to(dt))
+    dx, dw, db = m.dense_grad(new(0, 5), new(5, 7), new(0, 7), biases=b, activation="relu", preact=new(0, 7))
+    assert dx.shape == (0, 5) and torch.equal(dw, torch.zeros(5, 7, dtype=dt, device=gpu)) and torch.equal(db, torch.zeros_like(b))
+    dx, dw, db = m.dense_grad(new(3, 5), new(5, 0), new(3, 0), biases=new(0))
+    assert torch.equal(dx, torch.zeros(3, 5, dtype=dt, device=gpu)) and dw.shape == (5, 0) and db.shape == (0,)
+    dx, dw, db = m.dense_grad(new(3, 0), new(0, 7), r, biases=b)
+    assert dx.shape == (3, 0) and dw.shape == (0, 7)
+    _within(db, r.double().sum(0), _half(dt) * r.double().sum(0).abs() + 8 * U * r.double().abs().sum(0), "grad_biases")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_infinities_and_nans_stay_in_their_rows_and_columns(gpu, dt):
+    m = _mod()
+    for rows, cin, cout in ((70, 129, 65), (512, 256, 512), (3, 512, 256)):
+        x, w = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2)
+        clean = m.dense(x, w)
+        x[1, 3] = float("nan")
+        w[5, 7] = float("inf")
+        out = m.dense(x, w)
+        assert torch.isnan(out[1]).all()
+        assert not torch.isfinite(out[:, 7]).any()
+        keep = torch.ones_like(out, dtype=torch.bool)
+        keep[1] = False
+        keep[:, 7] = False
+        assert torch.equal(out[keep], clean[keep])
+        assert torch.isnan(m.dense(x, w, activation="relu")[1]).all()
+    # what reaches a closed ReLU does not come through, infinities included
+    z = torch.tensor([[-1.0, 0.0, 2.0, -3.0]], device=gpu).to(dt)
+    g = torch.tensor([[float("inf"), float("nan"), 1.0, 2.0]], device=gpu).to(dt)
+    x, w = torch.ones(1, 2, dtype=dt, device=gpu), torch.ones(2, 4, dtype=dt, device=gpu)
+    dx, dw, db = m.dense_grad(x, w, g, biases=torch.zeros(4, dtype=dt, device=gpu), activation="relu", preact=z)
+    assert db.tolist() == [0.0, 0.0, 1.0, 0.0] and dx.tolist() == [[1.0, 1.0]] and dw.tolist() == [[0.0, 0.0, 1.0, 0.0]] * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", [(5, 64, 40), (131, 67, 259), (300, 512, 264), (2048, 512, 128)])
+def test_nothing_is_written_outside_the_outputs(gpu, dt, size):
+    lib, m = pkg("utils._native").lib(), _mod()
+    rows, cin, cout = size
+    x, w, g, z = (_rand(gpu, s, dt, i) for i, s in enumerate(((rows, cin), (cin, cout), (rows, cout), (rows, cout))))
+    code = m.TYPES[dt]
+    guard = 4096
+
+    def padded(n):
+        t = torch.full((n + 2 * guard,), 7.0, dtype=dt, device=gpu)
+        return t, t[guard:guard + n]
+
+    def intact(t, n):
+        return bool((t[:guard] == 7).all()) and bool((t[guard + n:] == 7).all())
+
+    ws_all, st = {}, torch.cuda.current_stream().cuda_stream
+
+    def scratch(need):
+        t = torch.full((need + 8192,), 11, dtype=torch.uint8, device=gpu)
+        ws_all[need] = t
+        return t
+
+    al = lambda *ts: sum(1 << i for i, t in enumerate(ts) if t.data_ptr() % 16 == 0 and t.shape[1] * t.element_size() % 16 == 0)  # noqa: E731
+    n = ctypes.c_ulong()
+    assert lib.sa_dense_forward_ws(code, rows, cin, cout, al(x, w), ctypes.byref(n)) == 0
+    ws = scratch(n.value)
+    (yb, y), (pb, p) = padded(rows * cout), padded(rows * cout)
+    assert lib.sa_dense_forward(code, rows, cin, cout, x.data_ptr(), cin, w.data_ptr(), cout, None, 0, None, 0, 4, y.data_ptr(),
+                                p.data_ptr(), ws.data_ptr(), n.value, st) == 0
+    assert intact(yb, rows * cout) and intact(pb, rows * cout) and bool((ws[n.value:] == 11).all())
+    assert torch.equal(y.view(rows, cout), m.dense(x, w, activation="silu"))
+    assert lib.sa_dense_backward_ws(code, rows, cin, cout, 4, 7, al(x, w, g), ctypes.byref(n)) == 0
+    ws = scratch(n.value)
+    (xb, dx), (wb, dw), (bb, db) = padded(rows * cin), padded(cin * cout), padded(cout)
+    assert lib.sa_dense_backward(code, rows, cin, cout, x.data_ptr(), cin, w.data_ptr(), cout, g.data_ptr(), cout, z.data_ptr(),
+                                 cout, 4, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, ws.data_ptr(), n.value, st) == 0
+    assert intact(xb, rows * cin) and intact(wb, cin * cout) and intact(bb, cout) and bool((ws[n.value:] == 11).all())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gpu):
+    # 2^26 + 70 rows of 40 channels: element offsets pass 2^31, byte offsets 2^32
+    m = _mod()
+    rows, cin, cout = (1 << 26) + 70, 40, 8
+    x = torch.zeros(rows, cin, dtype=torch.bfloat16, device=gpu)
+    w = _rand(gpu, (cin, cout), torch.bfloat16, 1)
+    x[-100:] = _rand(gpu, (100, cin), torch.bfloat16, 2)
+    out = m.dense(x, w)
+    _check_forward(x[-100:], w, None, None, None, out[-100:], None)
+    assert not bool(out[:-100].any())
+    _, dw, _ = m.dense_grad(x, w, out, needs=(False, True))
+    _check_grad(x[-100:], w, out[-100:], None, None, None, dw, None)
+
+
+# ------------------------------------------------------------------------------------------- GPU: streams, graphs, refusals
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_other_streams_and_captured_graphs_give_the_same_bits(gpu, dt):
+    m = _mod()
+    for rows, cin, cout in ((1, 1024, 512), (515, 771, 259), (512, 512, 512)):
+        x, w, b = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2, 0.05), _rand(gpu, (cout,), dt, 3)
+        g = _rand(gpu, (rows, cout), dt, 4)
+
+        def step():
+            out, z = m.dense(x, w, b, activation="gelu", return_preact=True)
+            return (out, z) + m.dense_grad(x, w, g, biases=b, activation="gelu", preact=z)
+
+        want = [t.clone() for t in step()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b_) for a, b_ in zip(other, want))
+        graphs = []
+        for _ in range(2):                             # two graphs of the same step, replayed in turn
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                outs = step()
+            graphs.append((gr, outs))
+        for turn in range(3):
+            x.copy_(_rand(gpu, x.shape, dt, 10 + turn))
+            eager = [t.clone() for t in step()]
+            for gr, outs in graphs:
+                gr.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(a, b_) for a, b_ in zip(outs, eager))
+
+
+@pytest.mark.gpu
+def test_refused_arguments(gpu):
+    m = _mod()
+    x, w, g = torch.zeros(4, 6, device=gpu), torch.zeros(6, 8, device=gpu), torch.zeros(4, 8, device=gpu)
+    for bad in (dict(inputs=x.double()), dict(inputs=x.int()), dict(weights=w.half()), dict(weights=w[:5]), dict(weights=w[None]),
+                dict(biases=torch.zeros(7, device=gpu)), dict(biases=torch.zeros(8, device=gpu).half()), dict(biases=torch.zeros(8)),
+                dict(residual=torch.zeros(4, 7, device=gpu)), dict(residual=g.half()), dict(activation="tanh"),
+                dict(inputs=torch.zeros((), device=gpu)), dict(residual=torch.zeros(1, 8, device=gpu))):
+        with pytest.raises(ValueError):
+            m.dense(**{**dict(inputs=x, weights=w), **bad})
+    for bad in (dict(grad_out=g[:3]), dict(grad_out=g.half()), dict(activation="relu"), dict(activation="relu", preact=g[:, :7]),
+                dict(activation="relu", preact=g.cpu()), dict(needs=(True,))):
+        with pytest.raises(ValueError):
+            m.dense_grad(**{**dict(inputs=x, weights=w, grad_out=g), **bad})
+
+
+# ------------------------------------------------------------------------------------------------ GPU: as they are used
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_training_step_of_a_residual_block(gpu, dt):
+    """Two layers with a residual around them, their gradients, and the clipping of all of them, against 64-bit autograd on
+    the CPU.  16-bit: every intermediate is rounded to the type, half a step each; with some six roundings between input and
+    gradient of terms of one size, 16 half steps of the tensor's largest value cover them.  fp32: the sums' errors."""
+    m, c = _mod(), pkg("utils.tf_ops.gradients.tf_gradients")
+    rows, ch, wide = 96, 64, 200
+    x, w1, b1 = _rand(gpu, (rows, ch), dt, 1), _rand(gpu, (ch, wide), dt, 2, ch ** -0.5), _rand(gpu, (wide,), dt, 3, 0.1)
+    w2, b2, g = _rand(gpu, (wide, ch), dt, 4, wide ** -0.5), _rand(gpu, (ch,), dt, 5, 0.1), _rand(gpu, (rows, ch), dt, 6)
+    h, z = m.dense(x, w1, b1, activation="silu", return_preact=True)
+    y = m.dense(h, w2, b2, residual=x)
+    dh, dw2, db2 = m.dense_grad(h, w2, g, biases=b2)
+    dx, dw1, db1 = m.dense_grad(x, w1, dh, biases=b1, activation="silu", preact=z)
+    clipped, norm = c.clip_by_global_norm([dw1, db1, dw2, db2], 5.0)
+    t = [v.double().cpu().requires_grad_() for v in (x, w1, b1, w2, b2)]
+    yr = torch.nn.functional.silu(t[0] @ t[1] + t[2]) @ t[3] + t[4] + t[0]
+    grads = torch.autograd.grad(yr, t, g.double().cpu())
+    tol = 16 * _half(dt) if dt != torch.float32 else 2 * _sum_bound(wide) * 16
+
+    def close(got, want, what):
+        assert float((got.double().cpu() - want).abs().max()) <= tol * float(want.abs().max()), what
+
+    close(y, yr.detach(), "y")
+    close(dx + g, grads[0], "dx")                      # the residual's share is grad_out itself
+    ref = math.sqrt(sum(float(v.pow(2).sum()) for v in grads[1:]))
+    assert abs(float(norm) - ref) <= tol * ref and ref > 5.0
+    for got, want, what in zip(clipped, grads[1:], ("w1", "b1", "w2", "b2")):
+        close(got, want * (5.0 / ref), what)
