@@ -11,6 +11,7 @@
 // a lane ends with four consecutive columns of one output row.
 // Few tiles: the k range is cut into pieces (Product::splits), whose fp32 sums meet in join_kernel in piece order.
 #include "dense_common.h"
+#include "dense_tile.h"
 
 using namespace dense;
 
@@ -143,28 +144,59 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
     }
 }
 
-// ---- in front of a backward product: dZ = G act'(Z), and the column sums of dZ ------------------------------------------
+// ---- operands in front of a product ---------------------------------------------------------------------------------
+// One pass over a stored matrix [rows][cols], any stride and alignment, that writes what the products read:
+//   dZ = G act'(Z), where there is a Z (ReLU selects: what a closed unit receives, infinities among it, does not come
+//   through), and the column sums of dZ, taken before any rounding;
+//   a copy in the layer's type with 16-byte aligned rows, zeros behind the last column up to a multiple of 8 -- for the
+//   tile kernel, whose loads are 16 bytes wide.  dZ is rounded to the layer's type here: it is an operand of the same MFMAs
+//   as X and W;
+//   or, of a fp32 matrix, three bf16 planes x = h + m + l, each the rounded rest of the one before: 27 bits, so nothing of
+//   x's 24 is lost, and the six products h h, h m, m h, m m, h l, l h of two such operands leave out terms below 2^-24 of
+//   the product -- fp32's own rounding -- at 6 / 16 of the cost of fp32 MFMAs.
 // A thread owns eight columns of every eighth row of its block's strip; the eight row lanes of a block meet in LDS, the
-// strips in sum_strips_kernel, both in a fixed order.  dZ is rounded to the layer's type, since the products read it as an
-// operand of the same MFMAs as X and W (the sums for the bias are taken before the rounding).
-struct Slope {
+// strips in sum_strips_kernel, in a fixed order.  Bound by memory: each element is read and written once.
+struct Job {
     const void *g, *z;    // z null: no activation
     long ldg, ldz;
     int vec;              // g and z: 16-byte aligned bases and rows
     int act;
     long rows;
     int cols;
-    void *dz;             // [rows][ldd] in the layer's type, ldd = cols rounded up to 8, zeros behind the last column; null: sums only
-    long ldd;
+    void *dst;            // [rows][ldd], or null: sums only
+    long ldd;             // cols rounded up to a multiple of 8
+    long plane;           // elements between planes; 0: one copy in the layer's type
     float *sums;          // [strips][cols], or null
     long strip;           // rows of a block
 };
+struct Jobs {
+    Job j[3];
+    long first[4];        // blocks of the jobs
+};
+
+// x finite and too large for bf16 rounds to its largest value (the planes below hold the rest); an infinity has no rest
+__device__ __forceinline__ void three_planes(float x, unsigned short (&o)[3]) {
+    float r = x;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        unsigned short h = from_f32<bf16_t>(r).u;
+        if ((h & 0x7fff) == 0x7f80 && fabsf(r) <= 3.402823466e38f) h -= 1;
+        o[i] = h;
+        const float f = __uint_as_float((unsigned)h << 16);
+        r = fabsf(f) <= 3.402823466e38f ? r - f : (f != f ? f : 0.0f);
+    }
+}
 
 template <class T>
-__global__ __launch_bounds__(256) void slope_kernel(Slope S) {
+__global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
     __shared__ float part[8][256 + 4];
-    const int c0 = blockIdx.x * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
-    const long r0 = (long)blockIdx.y * S.strip, r1 = r0 + S.strip < S.rows ? r0 + S.strip : S.rows;
+    const int which = blockIdx.x >= J.first[2] ? 2 : blockIdx.x >= J.first[1] ? 1 : 0;
+    const Job S = J.j[which];
+    const long blk = blockIdx.x - J.first[which];
+    const int cb = (S.cols + 255) / 256, bx = (int)(blk % cb);
+    const long by = blk / cb;
+    const int c0 = bx * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    const long r0 = by * S.strip, r1 = r0 + S.strip < S.rows ? r0 + S.strip : S.rows;
     float sum[8] = {};
     if (c0 < S.cols) {
         for (long r = r0 + rl; r < r1; r += 8) {
@@ -177,16 +209,28 @@ __global__ __launch_bounds__(256) void slope_kernel(Slope S) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float zi = to_f32<T>(z.x[i]);
-                    // ReLU selects: what a closed unit receives, infinities among it, does not come through
                     if (S.act == kRelu) d[i] = zi > 0.0f ? d[i] : (zi != zi ? zi : 0.0f);
                     else d[i] = c0 + i < S.cols ? d[i] * act_slope(zi, S.act) : 0.0f;
                 }
             }
-            if (S.dz) {
-                Eight<T> o;
+            if (S.dst) {
+                if (sizeof(T) == 4 && S.plane) {
+                    Eight<bf16_t> o[3];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
-                *(Eight<T> *)((T *)S.dz + r * S.ldd + c0) = o;
+                    for (int i = 0; i < 8; ++i) {
+                        unsigned short h[3];
+                        three_planes(d[i], h);
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) o[p].x[i].u = h[p];
+                    }
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) *(Eight<bf16_t> *)((bf16_t *)S.dst + p * S.plane + r * S.ldd + c0) = o[p];
+                } else {
+                    Eight<T> o;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
+                    *(Eight<T> *)((T *)S.dst + r * S.ldd + c0) = o;
+                }
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += d[i];
@@ -196,11 +240,11 @@ __global__ __launch_bounds__(256) void slope_kernel(Slope S) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[rl][(threadIdx.x & 31) * 8 + i] = sum[i];
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int c = bx * 256 + threadIdx.x;
     if (c < S.cols) {
         float s = part[0][threadIdx.x];
         for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-        S.sums[(long)blockIdx.y * S.cols + c] = s;
+        S.sums[by * S.cols + c] = s;
     }
 }
 
@@ -218,44 +262,7 @@ __global__ __launch_bounds__(256) void sum_strips_kernel(const float *sums, int 
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 inline long esize(int type) { return type == kF32 ? 4 : 2; }
-inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0; }
-
-// Pieces of the k range: enough workgroups for two per CU, at least 128 k indices each.
-inline void split(Product &P) {
-    const long tiles = ((P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT);
-    long s = (512 + tiles - 1) / tiles;
-    const long most = P.K / 128;
-    if (s > most) s = most;
-    if (s < 1) s = 1;
-    P.kchunk = round_up((P.K + s - 1) / s, kStep);
-    if (P.kchunk < kStep) P.kchunk = kStep;
-    P.splits = (int)((P.K + P.kchunk - 1) / P.kchunk);
-    if (P.splits < 1) P.splits = 1;
-}
-inline unsigned long part_bytes(const Product &P) {
-    return P.splits > 1 ? (unsigned long)P.splits * P.M * round_up(P.N, 4) * 4 : 0;
-}
-
-template <class T, bool TA, bool TB>
-int launch(const Product &P, hipStream_t s) {
-    const long tiles = ((P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT);
-    if (tiles > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((product_kernel<T, TA, TB>), dim3((unsigned)tiles, P.splits), dim3(256), 0, s, P);
-    SA_CHECK_LAUNCH();
-    if (P.splits > 1) {
-        const long blocks = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
-        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, P);
-        SA_CHECK_LAUNCH();
-    }
-    return SA_OK;
-}
-template <bool TA, bool TB>
-int launch(int type, const Product &P, hipStream_t s) {
-    if (type == kF32) return launch<float, TA, TB>(P, s);
-    if (type == kBF16) return launch<bf16_t, TA, TB>(P, s);
-    return launch<f16_t, TA, TB>(P, s);
-}
-
+inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld < kMaxLd; }
 inline bool sizes_ok(int type, long rows, int cin, int cout) {
     return type >= kF32 && type <= kF16 && rows >= 0 && cin >= 0 && cout >= 0;
 }
@@ -272,66 +279,168 @@ struct Scratch {
     }
 };
 
-Product forward_product(long rows, int cin, int cout) {
-    Product P{};
-    P.M = rows; P.N = cout; P.K = cin;
-    split(P);
-    return P;
+// A stored matrix: an operand of one or two products.
+struct Matrix {
+    const void *p;
+    long ld, rows;
+    int cols;
+    bool vec;             // 16-byte aligned base and rows, fewer than kMaxLd elements apart
+    long plane = 0;
+};
+
+constexpr double kTileWork = 1 << 26;
+// Does a layer of this size go to the tile kernel?
+inline bool wants_tiles(int type, long rows, int cin, int cout) {
+    return rows >= 32 && cin >= 32 && cout >= 32 && (double)rows * cin * cout >= kTileWork && cin < kMaxLd && cout < kMaxLd;
+}
+// The tile kernel's loads are 16 bytes of 16-bit elements
+inline bool tile_operand(int type, const Matrix &m) { return type != kF32 && m.vec && m.cols % 8 == 0; }
+
+// Makes the copy (or planes) of m that the products read, as one of J's jobs
+void add_job(Jobs &J, int &n, Job j) {
+    J.j[n] = j;
+    J.first[n + 1] = J.first[n] + (long)((j.cols + 255) / 256) * ((j.rows + j.strip - 1) / j.strip);
+    ++n;
+}
+void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
+    Job j{};
+    j.g = m.p; j.ldg = m.ld; j.vec = m.vec; j.rows = m.rows; j.cols = m.cols;
+    j.ldd = round_up(m.cols, 8);
+    j.plane = type == kF32 ? m.rows * j.ldd : 0;
+    j.dst = ws.take((unsigned long)m.rows * j.ldd * 2 * (type == kF32 ? 3 : 1));
+    j.strip = 64;
+    m = Matrix{j.dst, j.ldd, m.rows, m.cols, true, j.plane};
+    add_job(J, n, j);
+}
+int launch_jobs(int type, Jobs &J, int n, hipStream_t s) {
+    if (n == 0 || J.first[n] == 0) return SA_OK;
+    if (J.first[n] > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    const unsigned blocks = (unsigned)J.first[n];
+    for (int i = n; i < 3; ++i) J.first[i] = J.first[i + 1] = 0x7fffffffL + 1;
+    if (type == kF32) hipLaunchKernelGGL((prepare_kernel<float>), dim3(blocks), dim3(256), 0, s, J);
+    else if (type == kBF16) hipLaunchKernelGGL((prepare_kernel<bf16_t>), dim3(blocks), dim3(256), 0, s, J);
+    else hipLaunchKernelGGL((prepare_kernel<f16_t>), dim3(blocks), dim3(256), 0, s, J);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+
+// A product and its k pieces.  64 x 64 tiles: two workgroups per CU, at least 128 k indices each.  Tile kernel: 256 x 256
+// tiles where they fill the chip, else 128 x 128, two workgroups per CU, at least four steps each.
+struct Plan {
+    Product P;
+    bool ta, tb;
+    int edge;             // 0: product_kernel
+};
+void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K) {
+    Product &P = L.P;
+    L.ta = ta; L.tb = tb;
+    P.M = M; P.N = N; P.K = K;
+    P.a = a.p; P.lda = a.ld; P.vec_a = a.vec; P.plane_a = a.plane;
+    P.b = b.p; P.ldb = b.ld; P.vec_b = b.vec; P.plane_b = b.plane;
+    P.passes = type == kF32 && tiles ? 6 : 1;
+    auto count = [&](long e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
+    L.edge = !tiles ? 0 : count(256) >= 192 ? 256 : 128;
+    const long unit = tiles ? 64 : kStep, steps = (K + unit - 1) / unit * P.passes, least = 4;
+    const long tilesn = count(tiles ? L.edge : kT), slots = L.edge == 256 ? 256 : 512;
+    long s = slots / tilesn;
+    if (s > steps / least) s = steps / least;
+    if (s < 1) s = 1;
+    long per = (steps + s - 1) / s;
+    if (per < 1) per = 1;
+    P.splits = (int)((steps + per - 1) / per);
+    if (P.splits < 1) P.splits = 1;
+    P.kchunk = tiles ? per : per * kStep;
+    P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * M * round_up(N, 4) * 4) : nullptr;
+}
+
+template <class T, bool TA, bool TB>
+int launch_product(const Product &P, hipStream_t s) {
+    const long tiles = ((P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT);
+    if (tiles > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((product_kernel<T, TA, TB>), dim3((unsigned)tiles, P.splits), dim3(256), 0, s, P);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+template <class T>
+int launch_plan(const Plan &L, hipStream_t s) {
+    const Product &P = L.P;
+    const int type = sizeof(T) == 4 ? kF32 : __is_same(T, bf16_t) ? kBF16 : kF16;
+    const int rc = L.edge ? launch_tiles(L.edge, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, P, s)
+                   : L.ta ? launch_product<T, true, true>(P, s)
+                   : L.tb ? launch_product<T, false, true>(P, s) : launch_product<T, false, false>(P, s);
+    if (rc || P.splits == 1) return rc;
+    const long blocks = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, P);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+int launch_plan(int type, const Plan &L, hipStream_t s) {
+    return type == kF32 ? launch_plan<float>(L, s) : type == kBF16 ? launch_plan<bf16_t>(L, s) : launch_plan<f16_t>(L, s);
+}
+
+struct Forward {
+    Jobs jobs;
+    int njobs;
+    Plan plan;
+};
+void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w) {
+    f = Forward{};
+    const bool tiles = wants_tiles(type, rows, cin, cout);
+    if (tiles) {
+        if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
+        if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
+    }
+    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin);
 }
 
 struct Backward {
-    Product dx, dw;
-    Slope slope;
+    Jobs jobs;
+    int njobs;
+    Plan dx, dw;
+    float *sums;
     int strips;
 };
 constexpr int kWantX = 1, kWantW = 2, kWantB = 4;
 
-void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, int act, int want) {
+void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w, Matrix g, Matrix z,
+                   int act, int want) {
     b = Backward{};
-    Slope &S = b.slope;
-    S.rows = rows; S.cols = cout; S.act = act;
-    S.strip = 64 * ((rows + 64 * 512 - 1) / (64 * 512));
-    if (S.strip < 64) S.strip = 64;
-    b.strips = (int)((rows + S.strip - 1) / S.strip);
-    S.ldd = round_up(cout, 8);
-    if (act != kNone && (want & (kWantX | kWantW))) S.dz = ws.take((unsigned long)rows * S.ldd * esize(type));
-    if (want & kWantB) S.sums = (float *)ws.take((unsigned long)b.strips * cout * 4);
-    if (want & kWantX) {
-        b.dx.M = rows; b.dx.N = cin; b.dx.K = cout;
-        split(b.dx);
-        b.dx.part = (float *)ws.take(part_bytes(b.dx));
+    const bool tiles = wants_tiles(type, rows, cin, cout), products = want & (kWantX | kWantW);
+    Job j{};
+    j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
+    j.vec = g.vec && (act == kNone || z.vec);
+    j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
+    j.strip = 64 * (rows / (64 * 512) + 1);            // at most 512 strips
+    Matrix d = g;
+    const bool copy = products && (act != kNone || (tiles && !tile_operand(type, g)));
+    if (copy) {
+        const bool planes = tiles && type == kF32;
+        j.dst = ws.take((unsigned long)rows * j.ldd * (planes ? 6 : esize(type)));
+        j.plane = planes ? rows * j.ldd : 0;
+        d = Matrix{j.dst, j.ldd, rows, cout, true, j.plane};
     }
-    if (want & kWantW) {
-        b.dw.M = cin; b.dw.N = cout; b.dw.K = rows;
-        split(b.dw);
-        b.dw.part = (float *)ws.take(part_bytes(b.dw));
+    if (want & kWantB) {
+        b.strips = (int)((rows + j.strip - 1) / j.strip);
+        j.sums = b.sums = (float *)ws.take((unsigned long)b.strips * cout * 4);
     }
-}
-
-template <class T>
-int launch_slope(const Backward &b, void *db, int db_f32, hipStream_t s) {
-    const Slope &S = b.slope;
-    if (S.rows > 0 && (S.dz || S.sums)) {
-        hipLaunchKernelGGL((slope_kernel<T>), dim3((S.cols + 255) / 256, b.strips), dim3(256), 0, s, S);
-        SA_CHECK_LAUNCH();
-    }
-    if (db) {
-        if (db_f32)
-            hipLaunchKernelGGL((sum_strips_kernel<float>), dim3((S.cols + 63) / 64), dim3(256), 0, s, S.sums, b.strips, S.cols,
-                               (float *)db);
-        else
-            hipLaunchKernelGGL((sum_strips_kernel<T>), dim3((S.cols + 63) / 64), dim3(256), 0, s, S.sums, b.strips, S.cols, (T *)db);
-        SA_CHECK_LAUNCH();
-    }
-    return SA_OK;
+    if (rows && cout && (copy || (want & kWantB))) add_job(b.jobs, b.njobs, j);
+    if (tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
+    if (tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
+    if (want & kWantX) plan(b.dx, ws, type, tiles, d, w, false, false, rows, cin, cout);
+    if (want & kWantW) plan(b.dw, ws, type, tiles, x, d, true, true, cin, cout, rows);
 }
 
 }  // namespace
 
 extern "C" int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes) {
-    (void)flags;
     if (!bytes || !sizes_ok(dtype, rows, cin, cout)) return SA_ERR_INVALID;
-    *bytes = rows && cout ? part_bytes(forward_product(rows, cin, cout)) : 0;
+    *bytes = 0;
+    if (rows == 0 || cout == 0) return SA_OK;
+    Forward f;
+    Scratch s{nullptr};
+    plan_forward(f, s, dtype, rows, cin, cout, Matrix{nullptr, cin, rows, cin, (flags & 1) != 0},
+                 Matrix{nullptr, cout, cin, cout, (flags & 2) != 0});
+    *bytes = s.used;
     return SA_OK;
 }
 
@@ -341,22 +450,25 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     if (!sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu) return SA_ERR_INVALID;
     if (rows == 0 || cout == 0) return SA_OK;
     if (!y || (cin && (!x || !w)) || ldx < cin || ldw < cout || (res && ldr < cout)) return SA_ERR_INVALID;
-    Product P = forward_product(rows, cin, cout);
-    P.a = x; P.lda = ldx; P.vec_a = aligned(x, ldx, dtype);
-    P.b = w; P.ldb = ldw; P.vec_b = aligned(w, ldw, dtype);
-    if (part_bytes(P) > ws_bytes || (part_bytes(P) && !ws)) return SA_ERR_INVALID;
-    P.part = (float *)ws;
-    P.e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act, 0};
-    P.e.vec = cout % 8 == 0 && aligned(y, cout, dtype) && (!pre || aligned(pre, cout, dtype)) && (!res || aligned(res, ldr, dtype));
-    return launch<false, true>(dtype, P, (hipStream_t)stream);
+    Forward f;
+    Scratch s{(char *)ws};
+    plan_forward(f, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
+                 Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)});
+    if (s.used > ws_bytes || (s.used && !ws)) return SA_ERR_INVALID;
+    Epilogue &e = f.plan.P.e;
+    e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act, 0};
+    e.vec = cout % 8 == 0 && aligned(y, cout, dtype) && (!pre || aligned(pre, cout, dtype)) && (!res || aligned(res, ldr, dtype));
+    const int rc = launch_jobs(dtype, f.jobs, f.njobs, (hipStream_t)stream);
+    return rc ? rc : launch_plan(dtype, f.plan, (hipStream_t)stream);
 }
 
 extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes) {
-    (void)flags;
     if (!bytes || !sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu || want < 0 || want > 7) return SA_ERR_INVALID;
     Backward b;
     Scratch s{nullptr};
-    plan_backward(b, s, dtype, rows, cin, cout, act, want);
+    plan_backward(b, s, dtype, rows, cin, cout, Matrix{nullptr, cin, rows, cin, (flags & 1) != 0},
+                  Matrix{nullptr, cout, cin, cout, (flags & 2) != 0}, Matrix{nullptr, cout, rows, cout, (flags & 4) != 0},
+                  Matrix{nullptr, cout, rows, cout, true}, act, want);
     *bytes = s.used;
     return SA_OK;
 }
@@ -372,33 +484,30 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     if ((want & kWantW) && rows && (!x || ldx < cin)) return SA_ERR_INVALID;
     Backward b;
     Scratch s{(char *)ws};
-    plan_backward(b, s, dtype, rows, cin, cout, act, want);
+    plan_backward(b, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
+                  Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)}, Matrix{g, ldg, rows, cout, aligned(g, ldg, dtype)},
+                  Matrix{z, ldz, rows, cout, aligned(z, ldz, dtype)}, act, want);
     if (s.used > ws_bytes || (s.used && !ws)) return SA_ERR_INVALID;
-    Slope &S = b.slope;
-    S.g = g; S.ldg = ldg;
-    S.z = act == kNone ? nullptr : z; S.ldz = ldz;
-    S.vec = aligned(g, ldg, dtype) && (!S.z || aligned(z, ldz, dtype));
     hipStream_t st = (hipStream_t)stream;
-    int rc = dtype == kF32 ? launch_slope<float>(b, want & kWantB ? db : nullptr, db_f32, st)
-             : dtype == kBF16 ? launch_slope<bf16_t>(b, want & kWantB ? db : nullptr, db_f32, st)
-                              : launch_slope<f16_t>(b, want & kWantB ? db : nullptr, db_f32, st);
+    int rc = launch_jobs(dtype, b.jobs, b.njobs, st);
     if (rc) return rc;
-    const void *dz = S.dz ? S.dz : g;
-    const long ldd = S.dz ? S.ldd : ldg;
-    const int vec_dz = aligned(dz, ldd, dtype);
+    if (want & kWantB) {
+        const dim3 grid((cout + 63) / 64);
+        if (db_f32 || dtype == kF32)
+            hipLaunchKernelGGL((sum_strips_kernel<float>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (float *)db);
+        else if (dtype == kBF16)
+            hipLaunchKernelGGL((sum_strips_kernel<bf16_t>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (bf16_t *)db);
+        else
+            hipLaunchKernelGGL((sum_strips_kernel<f16_t>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (f16_t *)db);
+        SA_CHECK_LAUNCH();
+    }
     if (want & kWantX) {
-        Product &P = b.dx;
-        P.a = dz; P.lda = ldd; P.vec_a = vec_dz;
-        P.b = w; P.ldb = ldw; P.vec_b = aligned(w, ldw, dtype);
-        P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cin % 8 == 0 && aligned(dx, cin, dtype)};
-        if ((rc = launch<false, false>(dtype, P, st))) return rc;
+        b.dx.P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cin % 8 == 0 && aligned(dx, cin, dtype)};
+        if ((rc = launch_plan(dtype, b.dx, st))) return rc;
     }
     if (want & kWantW) {
-        Product &P = b.dw;
-        P.a = x; P.lda = ldx; P.vec_a = aligned(x, ldx, dtype);
-        P.b = dz; P.ldb = ldd; P.vec_b = vec_dz;
-        P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cout % 8 == 0 && aligned(dw, cout, dtype)};
-        if ((rc = launch<true, true>(dtype, P, st))) return rc;
+        b.dw.P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cout % 8 == 0 && aligned(dw, cout, dtype)};
+        if ((rc = launch_plan(dtype, b.dw, st))) return rc;
     }
     return SA_OK;
 }

@@ -149,7 +149,9 @@ struct Product {
     long M, N, K;
     int vec_a, vec_b;     // 16-byte aligned base and rows
     int splits;           // the k range is cut into this many pieces, each summed by a workgroup of its own
-    long kchunk;          // k indices of one piece
+    long kchunk;          // k indices (tiles: steps) of one piece
+    int passes;           // tiles: 1, or 6 for fp32 operands in three bf16 planes each
+    long plane_a, plane_b;   // elements between planes
     float *part;          // splits > 1: [splits][M][Np] partial sums, Np = N rounded up to a multiple of 4
     Epilogue e;
 };

@@ -1,0 +1,233 @@
+// The large products of the dense layer: operands of 16-bit elements with 16-byte aligned rows (others are brought into
+// that form first, dense.hip).  D(m,n) = sum_k A(m,k) B(n,k), tiles of BM x BN per workgroup, k in steps of 64.
+//
+// Both operands go from memory straight into LDS (buffer loads with an LDS destination, 16 bytes per lane), into one of two
+// buffers while the products read the other.  A lane outside the operand gets an offset beyond the buffer's range, which
+// fills its 16 bytes with zeros: no edge of m, n or k needs code of its own, and nothing outside the operand is read.
+//   k contiguous      LDS rows of 64 k (128 bytes); the 16-byte pieces of a row are permuted by piece ^= row & 7, so that
+//                     ds_read_b128 of one piece of 16 rows touches all banks evenly.
+//   m / n contiguous  LDS rows of one k; 32-byte slots are permuted by slot ^= k (mod the number of slots), and the
+//                     fragments come through ds_read_b64_tr_b16, which transposes 4 k x 16 rows between the lanes.
+// The permutation costs nothing: a lane of the load picks which 16 bytes it fetches, the LDS side stays linear.
+#include "dense_common.h"
+#include "dense_tile.h"
+
+using namespace dense;
+
+namespace {
+
+constexpr int kBK = 64;
+constexpr unsigned kOutside = 0x80000000u;             // past every buffer's range
+
+typedef __attribute__((address_space(3))) char *lds_ptr;
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 *lds_s4;
+
+template <class MT> __device__ __forceinline__ f4 mfma(s8 a, s8 b, f4 c);
+template <> __device__ __forceinline__ f4 mfma<bf16_t>(s8 a, s8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f4 mfma<f16_t>(s8 a, s8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from buffer r + off to LDS `to` + 16 lane.  Written as assembly because the compiler, which knows the
+// builtin's loads by the LDS they write, waits for all of them in front of the next read of any LDS -- the other buffer's
+// included -- and the loads would never fly under the products.  Nothing comes back in registers; the kernel waits for
+// vmcnt itself, in front of the barrier that publishes the buffer.
+__device__ __forceinline__ void lds_load(u4 r, unsigned off, unsigned to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory", "m0");
+}
+
+// One operand's way into LDS: a tile of R rows x 64 k by W waves.
+template <int R, int W, bool ROWS>
+struct Loader {
+    static constexpr int kLoads = R * kBK * 2 / 1024 / W;      // 1024-byte loads per wave
+    static constexpr int kPieces = R / 8;                      // 16-byte pieces of one k (ROWS)
+    unsigned off[kLoads];
+    int k[kLoads];                                             // k of the lane's piece inside a step
+    __device__ __forceinline__ void init(int wave, int lane, long ld, long rows_left) {
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+            const int j = wave * kLoads + q;                   // which kilobyte of the tile
+            if (ROWS) {
+                const int b = j * 1024 + lane * 16;
+                const int kk = b / (R * 2), p = (b >> 4) & (kPieces - 1);
+                const int piece = p ^ (2 * (kk & (kPieces / 2 - 1)));
+                k[q] = kk;
+                off[q] = piece * 8 < rows_left ? (unsigned)(kk * ld * 2 + piece * 16) : kOutside;
+            } else {
+                const int row = j * 8 + (lane >> 3), piece = (lane & 7) ^ (row & 7);
+                k[q] = piece * 8;
+                off[q] = row < rows_left ? (unsigned)(row * ld * 2 + piece * 16) : kOutside;
+            }
+        }
+    }
+    // base: the tile's first row at this step's first k; k_left: valid k indices from there
+    __device__ __forceinline__ void load(const char *base, int k_left, char *lds, int wave) const {
+        const u4 r = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffff, 0x7fffffffu, 0x00020000u};
+        const unsigned to = (unsigned)(uintptr_t)(lds_ptr)(lds + wave * kLoads * 1024);
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) lds_load(r, k[q] < k_left ? off[q] : kOutside, to + q * 1024);
+    }
+};
+
+// Fragments of a wave: F blocks of 16 rows from row `first` on, 32 k each (half s of the step)
+template <int R, int F, bool ROWS>
+struct Reader {
+    int at[ROWS ? F : 2];
+    __device__ __forceinline__ void init(int first, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        if (ROWS) {
+            constexpr int slots = R / 16;
+            const int kk = 8 * g + (i >> 2);
+#pragma unroll
+            for (int f = 0; f < F; ++f) at[f] = kk * R * 2 + (((first / 16 + f) ^ (kk & (slots - 1))) * 32) + (i & 3) * 8;
+        } else {
+            at[0] = (first + i) * 128 + ((g ^ (i & 7)) * 16);
+            at[1] = (first + i) * 128 + (((g + 4) ^ (i & 7)) * 16);
+        }
+    }
+    __device__ __forceinline__ s8 read(const char *lds, int f, int s) const {
+        if (ROWS) {
+            // k + 4 flips bit 2 of the slot permutation: the same place as block f ^ 4 four rows on (F >= 8), or computed
+            const char *p = lds + at[f] + s * 32 * R * 2;
+            const char *p2 = lds + (at[f] ^ 128) + s * 32 * R * 2 + 4 * R * 2;
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p2);
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return *(const s8 *)(lds + at[s] + f * 2048);
+    }
+};
+
+// Planes of a fp32 operand (dense.hip): which plane of A meets which of B, the smallest terms first
+__device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
+
+template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB>
+__global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : WM * WN / 2) void tile_kernel(Product P) {
+    constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, kA = BM * kBK * 2, kB = BN * kBK * 2;
+    static_assert(FN == 4 && FM % 4 == 0 && W * 16384 <= 2 * (kA + kB), "the epilogue takes 64 x 64 of a wave at a time");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * (kA + kB)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // tiles in groups of eight tile rows, each XCD a contiguous run of them: neighbours share operands in one L2
+    const unsigned tm = (unsigned)((P.M + BM - 1) / BM), tn = (unsigned)((P.N + BN - 1) / BN), total = tm * tn;
+    const unsigned q8 = total >> 3, r8 = total & 7, xcd = blockIdx.x & 7;
+    const unsigned pos = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+    const unsigned group = pos / (8 * tn), in = pos - group * 8 * tn, rows = tm - group * 8 < 8 ? tm - group * 8 : 8;
+    const long m0 = (long)(group * 8 + in % rows) * BM, n0 = (long)(in / rows) * BN;
+
+    Loader<BM, W, TA> la;
+    Loader<BN, W, TB> lb;
+    la.init(wave, lane, P.lda, P.M - m0);
+    lb.init(wave, lane, P.ldb, P.N - n0);
+    Reader<BM, FM, TA> ra;
+    Reader<BN, FN, TB> rb;
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    ra.init(wm, lane);
+    rb.init(wn, lane);
+
+    const long per = (P.K + kBK - 1) / kBK;            // steps of one pass over k
+    const long first = (long)blockIdx.y * P.kchunk, steps = per * P.passes;
+    const long last = first + P.kchunk < steps ? first + P.kchunk : steps;
+    const char *A = (const char *)P.a + (TA ? m0 : m0 * P.lda) * 2, *B = (const char *)P.b + (TB ? n0 : n0 * P.ldb) * 2;
+    const long stepa = (TA ? P.lda : 1) * kBK * 2, stepb = (TB ? P.ldb : 1) * kBK * 2;
+
+    auto issue = [&](long step, char *to) {
+        const long pass = P.passes == 1 ? 0 : step / per, k = P.passes == 1 ? step : step - pass * per;
+        const char *a = A + k * stepa, *b = B + k * stepb;
+        if (P.passes > 1) {
+            a += kPlaneA[pass] * P.plane_a * 2;
+            b += kPlaneB[pass] * P.plane_b * 2;
+        }
+        const long left = P.K - k * kBK;
+        la.load(a, left < kBK ? (int)left : kBK, to, wave);
+        lb.load(b, left < kBK ? (int)left : kBK, to + kA, wave);
+    };
+
+    f4 acc[FN][FM] = {};
+    if (first < last) issue(first, lds);
+    for (long step = first; step < last; ++step) {
+        char *cur = lds + (int)((step - first) & 1) * (kA + kB), *nxt = lds + (int)((step - first + 1) & 1) * (kA + kB);
+        __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0): this wave's part of the step has arrived
+        __syncthreads();                               // and every wave's; nobody reads the other buffer any more
+        if (step + 1 < last) issue(step + 1, nxt);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            s8 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = ra.read(cur, i, s);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = rb.read(cur + kA, j, s);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[j][i] = mfma<MT>(fb[j], fa[i], acc[j][i]);
+        }
+    }
+
+    // The sums leave through LDS, 64 x 64 of a wave at a time (16 KB of its own): the epilogue's code then exists once, and
+    // eight lanes write 128 neighbouring bytes (16-bit) of a row.  16-byte pieces of a row are permuted by ^ row & 15.
+    const long Np = round_up(P.N, 4);
+    char *mine = lds + wave * 16384;
+    const long n = n0 + wn + (lane & 7) * 8;
+    float bias[8];
+    load_bias<OT, 8>(P.e, n, P.N, bias);               // (none in a product whose sums are joined later: unused there)
+    __syncthreads();
+#pragma unroll 1
+    for (int h = 0; h < FM / 4; ++h) {
+#pragma unroll
+        for (int hh = 0; hh < FM / 4; ++hh)
+            if (hh == h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = 16 * i + (lane & 15), piece = (4 * j + (lane >> 4)) ^ (lane & 15);
+                        *(f4 *)(mine + row * 256 + piece * 16) = acc[j][4 * hh + i];
+                    }
+            }
+#pragma unroll 1
+        for (int q = 0; q < 8; ++q) {
+            const int row = q * 8 + (lane >> 3), piece = (lane & 7) * 2;
+            const f4 lo = *(const f4 *)(mine + row * 256 + ((piece ^ (row & 15)) * 16));
+            const f4 hi = *(const f4 *)(mine + row * 256 + (((piece + 1) ^ (row & 15)) * 16));
+            const long m = m0 + wm + 64 * h + row;
+            if (m >= P.M || n >= P.N) continue;
+            if (P.splits > 1) {
+                float *p = P.part + ((long)blockIdx.y * P.M + m) * Np + n;
+                *(f4 *)p = lo;
+                if (n + 4 < P.N) *(f4 *)(p + 4) = hi;
+            } else {
+                const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                finish<OT, 8>(P.e, m, n, P.N, v, bias);
+            }
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN, class MT, class OT>
+int launch(bool ta, bool tb, const Product &P, hipStream_t s) {
+    const long tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
+    if (tiles > 0x3fffffffL) return SA_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)tiles, P.splits), block(WM * WN * 64);
+    if (ta) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, true, true>), grid, block, 0, s, P);
+    else if (tb) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, true>), grid, block, 0, s, P);
+    else hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, false>), grid, block, 0, s, P);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+
+template <class MT, class OT>
+int launch(int edge, bool ta, bool tb, const Product &P, hipStream_t s) {
+    if (edge == 256) return launch<256, 256, 2, 4, MT, OT>(ta, tb, P, s);
+    return launch<128, 128, 2, 2, MT, OT>(ta, tb, P, s);
+}
+
+}  // namespace
+
+int dense::launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s) {
+    if (out_type == kF32) return launch<bf16_t, float>(edge, ta, tb, P, s);
+    if (type == kBF16) return launch<bf16_t, bf16_t>(edge, ta, tb, P, s);
+    return launch<f16_t, f16_t>(edge, ta, tb, P, s);
+}

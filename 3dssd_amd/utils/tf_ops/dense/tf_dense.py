@@ -73,7 +73,7 @@ def _layer(op, inputs, weights, biases, activation):
 
 
 def _aligned(ptr, ld, itemsize):
-    return ptr % 16 == 0 and ld * itemsize % 16 == 0
+    return ptr % 16 == 0 and ld * itemsize % 16 == 0 and ld < 1 << 21
 
 
 def dense(inputs, weights, biases=None, activation=None, residual=None, return_preact=False):

@@ -256,8 +256,8 @@ int sa_dense(long rows, int K, int N, const float *x, const void *wpack, const f
  * (ldw), res [rows,cout] (ldr; nullable), y and pre [rows,cout] (dense; pre = x W + bias, nullable); bias [cout] (nullable)
  * is fp32 where bias_f32 is set, else of that type.  act: 0 none, 1 ReLU, 2 GELU (normal integral), 3 GELU (tanh form),
  * 4 SiLU.  Any sizes, strides and alignments of whole elements; sums in fp32, one rounding per output, no atomics: the
- * same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has 16-byte aligned base and
- * rows), 16-byte aligned, used until the call's work on the stream is done. */
+ * same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has a 16-byte aligned base
+ * and rows, fewer than 2^21 elements apart), 256-byte aligned, used until the call's work on the stream is done. */
 int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes);
 int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
                      const void *bias, int bias_f32, const void *res, long ldr, int act, void *y, void *pre, void *ws,
@@ -265,7 +265,7 @@ int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, lon
 /* Gradient: dz = g act'(z), dx = dz W^T [rows,cin], dw = x^T dz [cin,cout], db = column sums of dz [cout] (fp32 where
  * db_f32), each nullable and dense; g, z [rows,cout] (ldg, ldz; z = pre of the forward call, unused with act 0).  16-bit
  * types round dz once, as an operand of the products.  want (of the _ws call): bit 0 / 1 / 2 = dx / dw / db; flags: bit
- * 0 / 1 / 2 = x / W / g has 16-byte aligned base and rows. */
+ * 0 / 1 / 2 = x / W / g is aligned as above. */
 int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes);
 int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
                       const void *g, long ldg, const void *z, long ldz, int act, void *dx, void *dw, void *db, int db_f32,
