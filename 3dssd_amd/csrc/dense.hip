@@ -1,15 +1,6 @@
 // The dense layer on plain weights: y = act(x W + b) + residual in fp32, bf16 or fp16, and its gradient
-// (dense_common.h has the formulas).  This file: the product kernel that takes any size, stride and alignment, the
-// pass in front of a backward product (dZ = G act'(Z) and its column sums), the join of split sums, and the C ABI.
-//
-// product_kernel: a workgroup of four waves owns a 64 x 64 tile of D and walks k in steps of 32.  Both operands go through
-// registers into LDS in [row][k] order whatever their layout in memory -- one step ahead of the products, so the loads of
-// a step fly while the last one is multiplied -- and come back as 16-byte fragments (rows padded to 80 / 144 bytes: eight
-// neighbouring rows start in eight different bank groups).  16-bit types run on v_mfma_f32_16x16x32, fp32 on
-// v_mfma_f32_16x16x4 (exact products, fp32 sums); a lane of the fp32 form reads four k values at once and gives them to
-// four MFMAs, which permutes k inside a step the same way on both sides.  The n index sits on the MFMA's row side, so that
-// a lane ends with four consecutive columns of one output row.
-// Few tiles: the k range is cut into pieces (Product::splits), whose fp32 sums meet in join_kernel in piece order.
+// (dense_common.h has the formulas).  This file: the pass in front of the products that need one, the join of split sums,
+// the choice of kernel, and the C ABI.  The products are in dense_tile.hip (large) and dense_small.hip.
 #include "dense_common.h"
 #include "dense_tile.h"
 
@@ -17,115 +8,19 @@ using namespace dense;
 
 namespace {
 
-constexpr int kT = 64, kStep = 32;                     // tile edge, k indices per step
-
-template <class T> struct Tile;
-template <> struct Tile<float> { static constexpr int ld = 36; };
-template <> struct Tile<bf16_t> { static constexpr int ld = 40; };
-template <> struct Tile<f16_t> { static constexpr int ld = 40; };
-
 template <class T> struct alignas(16) Eight { T x[8]; };
 
-// Eight neighbours in memory: elements (row, k .. k + 8) of an operand with k contiguous, or (row .. row + 8, k) of one
-// with rows contiguous; zeros outside [0, rows) x [0, kend).
-template <class T, bool ROWS>
-__device__ __forceinline__ Eight<T> fetch(const T *p, long ld, int vec, long row, long rows, long k, long kend) {
+// Columns c .. c + 8 of a row; zeros behind the last column.
+template <class T>
+__device__ __forceinline__ Eight<T> fetch(const T *row, int vec, int c, int cols) {
     Eight<T> v;
-    const long fast = ROWS ? row : k, nfast = ROWS ? rows : kend;
-    const bool in = ROWS ? k < kend : row < rows;
-    const T *q = p + (ROWS ? k * ld + row : row * ld + k);
-    if (vec && in && fast + 8 <= nfast) {
-        v = *(const Eight<T> *)q;
+    if (vec && c + 8 <= cols) {
+        v = *(const Eight<T> *)(row + c);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.x[i] = (in && fast + i < nfast) ? q[i] : T{};
+        for (int i = 0; i < 8; ++i) v.x[i] = c + i < cols ? row[c + i] : T{};
     }
     return v;
-}
-
-template <class T, bool ROWS>
-__device__ __forceinline__ void stage(T *lds, int t, const Eight<T> &v) {
-    constexpr int ld = Tile<T>::ld;
-    if (ROWS) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) lds[((t & 7) * 8 + i) * ld + (t >> 3)] = v.x[i];
-    } else {
-        *(Eight<T> *)(lds + (t >> 2) * ld + (t & 3) * 8) = v;
-    }
-}
-
-template <class T>
-__device__ __forceinline__ f4 mfma_step(const T *a, const T *b, f4 c);   // a, b: fragment start of this lane's row
-template <>
-__device__ __forceinline__ f4 mfma_step<bf16_t>(const bf16_t *a, const bf16_t *b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const b8 *)a, *(const b8 *)b, c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f4 mfma_step<f16_t>(const f16_t *a, const f16_t *b, f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8 *)a, *(const h8 *)b, c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f4 mfma_step<float>(const float *a, const float *b, f4 c) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {                      // k = 16 s + 4 (lane / 16) + j
-        const f4 x = *(const f4 *)(a + 16 * s), y = *(const f4 *)(b + 16 * s);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    }
-    return c;
-}
-
-template <class T, bool TA, bool TB>
-__global__ __launch_bounds__(256) void product_kernel(Product P) {
-    __shared__ T sa[kT * Tile<T>::ld], sb[kT * Tile<T>::ld];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const long tn = (P.N + kT - 1) / kT;
-    const long tile = blockIdx.x, m0 = tile / tn * kT, n0 = tile % tn * kT;
-    const long k0 = (long)blockIdx.y * P.kchunk, kend = k0 + P.kchunk < P.K ? k0 + P.kchunk : P.K;
-    const T *A = (const T *)P.a, *B = (const T *)P.b;
-    const long ra = m0 + (TA ? (t & 7) * 8 : t >> 2), rb = n0 + (TB ? (t & 7) * 8 : t >> 2);
-    const int ka = TA ? t >> 3 : (t & 3) * 8, kb = TB ? t >> 3 : (t & 3) * 8;
-    const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-    // this lane's k offset inside a fragment: eight 16-bit values or one float4
-    const int frag = (lane & 15) * Tile<T>::ld + (lane >> 4) * (sizeof(T) == 4 ? 4 : 8);
-    f4 acc[2][2] = {};
-    Eight<T> va{}, vb{};
-    if (k0 < kend) {
-        va = fetch<T, TA>(A, P.lda, P.vec_a, ra, P.M, k0 + ka, kend);
-        vb = fetch<T, TB>(B, P.ldb, P.vec_b, rb, P.N, k0 + kb, kend);
-    }
-    for (long k = k0; k < kend; k += kStep) {
-        stage<T, TA>(sa, t, va);
-        stage<T, TB>(sb, t, vb);
-        __syncthreads();
-        if (k + kStep < kend) {
-            va = fetch<T, TA>(A, P.lda, P.vec_a, ra, P.M, k + kStep + ka, kend);
-            vb = fetch<T, TB>(B, P.ldb, P.vec_b, rb, P.N, k + kStep + kb, kend);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                acc[j][i] = mfma_step<T>(sb + (wn + 16 * j) * Tile<T>::ld + frag, sa + (wm + 16 * i) * Tile<T>::ld + frag,
-                                         acc[j][i]);
-        __syncthreads();
-    }
-    const long Np = round_up(P.N, 4);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const long n = n0 + wn + 16 * j + (lane >> 4) * 4;
-        if (n >= P.N) continue;
-        float b[4];
-        if (P.splits == 1) load_bias<T, 4>(P.e, n, P.N, b);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const long m = m0 + wm + 16 * i + (lane & 15);
-            if (m >= P.M) continue;
-            const float v[4] = {acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]};
-            if (P.splits > 1) *(f4 *)(P.part + ((long)blockIdx.y * P.M + m) * Np + n) = acc[j][i];
-            else finish<T, 4>(P.e, m, n, P.N, v, b);
-        }
-    }
 }
 
 // The pieces of a split k range, summed in piece order, then the epilogue.
@@ -136,6 +31,7 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
         const long m = i / per, n = (i - m * per) * 4;
         const float *p = P.part + m * Np + n;
         f4 s = *(const f4 *)p;
+#pragma unroll 8
         for (int z = 1; z < P.splits; ++z) s += *(const f4 *)(p + z * plane);
         float b[4];
         load_bias<T, 4>(P.e, n, P.N, b);
@@ -198,22 +94,31 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
     const int c0 = bx * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
     const long r0 = by * S.strip, r1 = r0 + S.strip < S.rows ? r0 + S.strip : S.rows;
     float sum[8] = {};
-    if (c0 < S.cols) {
-        for (long r = r0 + rl; r < r1; r += 8) {
-            const Eight<T> g = fetch<T, false>((const T *)S.g, S.ldg, S.vec, r, S.rows, c0, S.cols);
+    constexpr int kRows = 4;                           // rows in flight per thread
+    for (long r = r0 + rl; r < r1 && c0 < S.cols; r += 8 * kRows) {
+        Eight<T> g[kRows], z[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+            if (r + 8 * u < r1) {
+                g[u] = fetch((const T *)S.g + (r + 8 * u) * S.ldg, S.vec, c0, S.cols);
+                if (S.z) z[u] = fetch((const T *)S.z + (r + 8 * u) * S.ldz, S.vec, c0, S.cols);
+            }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            if (r + 8 * u >= r1) break;
             float d[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = to_f32<T>(g.x[i]);
+            for (int i = 0; i < 8; ++i) d[i] = to_f32<T>(g[u].x[i]);
             if (S.z) {
-                const Eight<T> z = fetch<T, false>((const T *)S.z, S.ldz, S.vec, r, S.rows, c0, S.cols);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float zi = to_f32<T>(z.x[i]);
+                    const float zi = to_f32<T>(z[u].x[i]);
                     if (S.act == kRelu) d[i] = zi > 0.0f ? d[i] : (zi != zi ? zi : 0.0f);
                     else d[i] = c0 + i < S.cols ? d[i] * act_slope(zi, S.act) : 0.0f;
                 }
             }
             if (S.dst) {
+                const long at = (r + 8 * u) * S.ldd + c0;
                 if (sizeof(T) == 4 && S.plane) {
                     Eight<bf16_t> o[3];
 #pragma unroll
@@ -224,12 +129,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
                         for (int p = 0; p < 3; ++p) o[p].x[i].u = h[p];
                     }
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) *(Eight<bf16_t> *)((bf16_t *)S.dst + p * S.plane + r * S.ldd + c0) = o[p];
+                    for (int p = 0; p < 3; ++p) *(Eight<bf16_t> *)((bf16_t *)S.dst + p * S.plane + at) = o[p];
                 } else {
                     Eight<T> o;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
-                    *(Eight<T> *)((T *)S.dst + r * S.ldd + c0) = o;
+                    *(Eight<T> *)((T *)S.dst + at) = o;
                 }
             }
 #pragma unroll
@@ -253,8 +158,10 @@ __global__ __launch_bounds__(256) void sum_strips_kernel(const float *sums, int 
     __shared__ float part[4][64];
     const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
     float s = 0.0f;
-    if (c < cols)
+    if (c < cols) {
+#pragma unroll 8
         for (int i = q; i < strips; i += 4) s += sums[(long)i * cols + c];
+    }
     part[q][threadIdx.x & 63] = s;
     __syncthreads();
     if (q == 0 && c < cols) out[c] = from_f32<T>((part[0][c & 63] + part[1][c & 63]) + (part[2][c & 63] + part[3][c & 63]));
@@ -262,9 +169,9 @@ __global__ __launch_bounds__(256) void sum_strips_kernel(const float *sums, int 
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 inline long esize(int type) { return type == kF32 ? 4 : 2; }
-inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld < kMaxLd; }
+inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld < kMaxTileLd; }
 inline bool sizes_ok(int type, long rows, int cin, int cout) {
-    return type >= kF32 && type <= kF16 && rows >= 0 && cin >= 0 && cout >= 0;
+    return type >= kF32 && type <= kF16 && rows >= 0 && cin >= 0 && cout >= 0 && cin < kMaxLd && cout < kMaxLd;
 }
 
 // Scratch of a call, piece by piece at 256-byte steps.  With base null only the size is counted.
@@ -284,17 +191,20 @@ struct Matrix {
     const void *p;
     long ld, rows;
     int cols;
-    bool vec;             // 16-byte aligned base and rows, fewer than kMaxLd elements apart
+    bool vec;             // 16-byte aligned base and rows, fewer than kMaxTileLd elements apart
     long plane = 0;
 };
 
-constexpr double kTileWork = 1 << 26;
-// Does a layer of this size go to the tile kernel?
-inline bool wants_tiles(int type, long rows, int cin, int cout) {
-    return rows >= 32 && cin >= 32 && cout >= 32 && (double)rows * cin * cout >= kTileWork && cin < kMaxLd && cout < kMaxLd;
-}
 // The tile kernel's loads are 16 bytes of 16-bit elements
 inline bool tile_operand(int type, const Matrix &m) { return type != kF32 && m.vec && m.cols % 8 == 0; }
+
+// Does a layer of this size go to the tile kernel?  The small kernel's time against the tiles' (us): fp32 512^3 8 / 24,
+// 1024^3 41 / 39, 2048 x 1024 x 1024 77 / 55; bf16 512^3 7 / 12, 1024 x 512 x 512 12 / 13, 1024^3 25 / 22; where the operands
+// have to be copied first 511^3 11 / 15, 1023^3 70 / 27.  A tile of 128 rows is no place for 32.
+inline bool wants_tiles(int type, long rows, int cin, int cout, bool copies) {
+    const double least = type == kF32 ? 1L << 30 : copies ? 1L << 28 : 1L << 29;
+    return rows > 32 && cin > 32 && cout > 32 && (double)rows * cin * cout >= least && cin < kMaxTileLd && cout < kMaxTileLd;
+}
 
 // Makes the copy (or planes) of m that the products read, as one of J's jobs
 void add_job(Jobs &J, int &n, Job j) {
@@ -302,13 +212,20 @@ void add_job(Jobs &J, int &n, Job j) {
     J.first[n + 1] = J.first[n] + (long)((j.cols + 255) / 256) * ((j.rows + j.strip - 1) / j.strip);
     ++n;
 }
+// Rows of a block: a thousand blocks where the matrix has them, and no more strips than 512
+long strip_of(long rows, int cols) {
+    long s = rows * ((cols + 255) / 256) / 1024;
+    if (s > 63) s = 63;
+    if (s < rows / 512) s = rows / 512;
+    return round_up(s + 1, 8);
+}
 void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
     Job j{};
     j.g = m.p; j.ldg = m.ld; j.vec = m.vec; j.rows = m.rows; j.cols = m.cols;
     j.ldd = round_up(m.cols, 8);
     j.plane = type == kF32 ? m.rows * j.ldd : 0;
     j.dst = ws.take((unsigned long)m.rows * j.ldd * 2 * (type == kF32 ? 3 : 1));
-    j.strip = 64;
+    j.strip = strip_of(m.rows, m.cols);
     m = Matrix{j.dst, j.ldd, m.rows, m.cols, true, j.plane};
     add_job(J, n, j);
 }
@@ -324,12 +241,12 @@ int launch_jobs(int type, Jobs &J, int n, hipStream_t s) {
     return SA_OK;
 }
 
-// A product and its k pieces.  64 x 64 tiles: two workgroups per CU, at least 128 k indices each.  Tile kernel: 256 x 256
-// tiles where they fill the chip, else 128 x 128, two workgroups per CU, at least four steps each.
+// A product and its k pieces.  Tiles: 256 x 256 where they fill the chip, else 128 x 128, two workgroups per CU, at least
+// eight steps each.  Small: blocks of 32 x 32, two workgroups per CU, at least 2048 k each (sixteen waves, four steps).
 struct Plan {
     Product P;
     bool ta, tb;
-    int edge;             // 0: product_kernel
+    int edge;             // 0: launch_small
 };
 void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K) {
     Product &P = L.P;
@@ -340,34 +257,25 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     P.passes = type == kF32 && tiles ? 6 : 1;
     auto count = [&](long e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
     L.edge = !tiles ? 0 : count(256) >= 192 ? 256 : 128;
-    const long unit = tiles ? 64 : kStep, steps = (K + unit - 1) / unit * P.passes, least = 4;
-    const long tilesn = count(tiles ? L.edge : kT), slots = L.edge == 256 ? 256 : 512;
-    long s = slots / tilesn;
+    const long steps = (K + 31) / 32 * P.passes, least = tiles ? 8 : 64;
+    const long blocks = count(tiles ? L.edge : 32), slots = L.edge == 256 ? 256 : 512;
+    long s = slots / blocks;
     if (s > steps / least) s = steps / least;
     if (s < 1) s = 1;
     long per = (steps + s - 1) / s;
     if (per < 1) per = 1;
     P.splits = (int)((steps + per - 1) / per);
     if (P.splits < 1) P.splits = 1;
-    P.kchunk = tiles ? per : per * kStep;
+    P.kchunk = tiles ? per : per * 32;
     P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * M * round_up(N, 4) * 4) : nullptr;
 }
 
-template <class T, bool TA, bool TB>
-int launch_product(const Product &P, hipStream_t s) {
-    const long tiles = ((P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT);
-    if (tiles > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((product_kernel<T, TA, TB>), dim3((unsigned)tiles, P.splits), dim3(256), 0, s, P);
-    SA_CHECK_LAUNCH();
-    return SA_OK;
-}
 template <class T>
 int launch_plan(const Plan &L, hipStream_t s) {
     const Product &P = L.P;
     const int type = sizeof(T) == 4 ? kF32 : __is_same(T, bf16_t) ? kBF16 : kF16;
     const int rc = L.edge ? launch_tiles(L.edge, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, P, s)
-                   : L.ta ? launch_product<T, true, true>(P, s)
-                   : L.tb ? launch_product<T, false, true>(P, s) : launch_product<T, false, false>(P, s);
+                          : launch_small(type, L.ta, L.tb, P, s);
     if (rc || P.splits == 1) return rc;
     const long blocks = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, P);
@@ -385,7 +293,7 @@ struct Forward {
 };
 void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w) {
     f = Forward{};
-    const bool tiles = wants_tiles(type, rows, cin, cout);
+    const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
     if (tiles) {
         if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
@@ -405,12 +313,13 @@ constexpr int kWantX = 1, kWantW = 2, kWantB = 4;
 void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w, Matrix g, Matrix z,
                    int act, int want) {
     b = Backward{};
-    const bool tiles = wants_tiles(type, rows, cin, cout), products = want & (kWantX | kWantW);
+    const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
+    const bool products = want & (kWantX | kWantW);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
     j.vec = g.vec && (act == kNone || z.vec);
     j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
-    j.strip = 64 * (rows / (64 * 512) + 1);            // at most 512 strips
+    j.strip = strip_of(rows, cout);
     Matrix d = g;
     const bool copy = products && (act != kNone || (tiles && !tile_operand(type, g)));
     if (copy) {
@@ -450,6 +359,7 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     if (!sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu) return SA_ERR_INVALID;
     if (rows == 0 || cout == 0) return SA_OK;
     if (!y || (cin && (!x || !w)) || ldx < cin || ldw < cout || (res && ldr < cout)) return SA_ERR_INVALID;
+    if (ldx >= kMaxLd || ldw >= kMaxLd) return SA_ERR_UNSUPPORTED;
     Forward f;
     Scratch s{(char *)ws};
     plan_forward(f, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
@@ -482,6 +392,7 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     if (rows && cout && (!g || ldg < cout || (act != kNone && (!z || ldz < cout)))) return SA_ERR_INVALID;
     if ((want & kWantX) && cout && (!w || ldw < cout)) return SA_ERR_INVALID;
     if ((want & kWantW) && rows && (!x || ldx < cin)) return SA_ERR_INVALID;
+    if (((want & kWantX) && ldw >= kMaxLd) || ((want & kWantW) && ldx >= kMaxLd) || ldg >= kMaxLd) return SA_ERR_UNSUPPORTED;
     Backward b;
     Scratch s{(char *)ws};
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},

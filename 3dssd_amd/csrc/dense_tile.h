@@ -1,12 +1,17 @@
-// Interface between dense.hip and dense_tile.hip.
+// Interface between dense.hip and the kernels for large (dense_tile.hip) and small products (dense_small.hip).
 #pragma once
 #include "dense_common.h"
 
 namespace dense {
-// D = A B^T on tiles of edge x edge (128 or 256) of 16-bit operands with 16-byte aligned bases and rows, whole 16-byte
-// pieces along the contiguous index, and fewer than kMaxLd elements between neighbours of the other index (offsets inside
-// a tile are 31-bit).  type: kBF16 / kF16 of the operands; out_type: that, or kF32.  P.kchunk counts steps of 64 k over all
-// passes.  ta and not tb does not occur.
-constexpr long kMaxLd = 1L << 21;
+// Byte offsets inside a block are 31-bit: fewer than this many elements between neighbours of an operand's outer index for
+// the 256 rows of a tile, and for the 32 of a small block (and no row is longer).
+constexpr long kMaxTileLd = 1L << 21, kMaxLd = 1L << 24;
+
+// D = A B^T on tiles of edge x edge (128 or 256) of 16-bit operands with 16-byte aligned bases and rows, and whole 16-byte
+// pieces along the contiguous index.  type: kBF16 / kF16 of the operands; out_type: that, or kF32.  P.kchunk counts steps of
+// 32 k over all passes.  ta and not tb does not occur.
 int launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
+
+// Any product; P.kchunk counts k indices (a multiple of 32).
+int launch_small(int type, bool ta, bool tb, const Product &P, hipStream_t s);
 }  // namespace dense

@@ -1,14 +1,19 @@
 // The large products of the dense layer: operands of 16-bit elements with 16-byte aligned rows (others are brought into
-// that form first, dense.hip).  D(m,n) = sum_k A(m,k) B(n,k), tiles of BM x BN per workgroup, k in steps of 64.
+// that form first, dense.hip).  D(m,n) = sum_k A(m,k) B(n,k), tiles of BM x BN per workgroup, k in steps of 32.
 //
-// Both operands go from memory straight into LDS (buffer loads with an LDS destination, 16 bytes per lane), into one of two
-// buffers while the products read the other.  A lane outside the operand gets an offset beyond the buffer's range, which
+// Both operands go from memory straight into LDS (buffer loads with an LDS destination, 16 bytes per lane), into a ring of
+// four buffers, three steps ahead of the products.  A lane outside the operand gets an offset beyond the buffer's range, which
 // fills its 16 bytes with zeros: no edge of m, n or k needs code of its own, and nothing outside the operand is read.
-//   k contiguous      LDS rows of 64 k (128 bytes); the 16-byte pieces of a row are permuted by piece ^= row & 7, so that
-//                     ds_read_b128 of one piece of 16 rows touches all banks evenly.
-//   m / n contiguous  LDS rows of one k; 32-byte slots are permuted by slot ^= k (mod the number of slots), and the
+//   k contiguous      LDS rows of 32 k (64 bytes); the 16-byte pieces of a row are permuted by piece ^= (row / 2) & 3, so that
+//                     ds_read_b128 of one piece of 8 rows touches all banks once.
+//   m / n contiguous  LDS rows of one k; 32-byte slots are permuted by three bits of k (slot_of), and the
 //                     fragments come through ds_read_b64_tr_b16, which transposes 4 k x 16 rows between the lanes.
 // The permutation costs nothing: a lane of the load picks which 16 bytes it fetches, the LDS side stays linear.
+//
+// 256 x 256: eight waves, two per SIMD, of 128 x 64 each (fragment reads 96 KB of LDS per step, 0.75 of what the products
+// take).  The second four run one phase behind the first: while one wave of a SIMD reads the fragments of a step, the other
+// has the matrix pipe to itself; a barrier ends every phase.  128 x 128: four waves of 64 x 64, two workgroups per CU, which
+// interleave by themselves.
 #include "dense_common.h"
 #include "dense_tile.h"
 
@@ -16,7 +21,7 @@ using namespace dense;
 
 namespace {
 
-constexpr int kBK = 64;
+constexpr int kBK = 32, kRing = 5;
 constexpr unsigned kOutside = 0x80000000u;             // past every buffer's range
 
 typedef __attribute__((address_space(3))) char *lds_ptr;
@@ -34,12 +39,16 @@ template <> __device__ __forceinline__ f4 mfma<f16_t>(s8 a, s8 b, f4 c) {
 // 16 bytes per lane from buffer r + off to LDS `to` + 16 lane.  Written as assembly because the compiler, which knows the
 // builtin's loads by the LDS they write, waits for all of them in front of the next read of any LDS -- the other buffer's
 // included -- and the loads would never fly under the products.  Nothing comes back in registers; the kernel waits for
-// vmcnt itself, in front of the barrier that publishes the buffer.
+// vmcnt itself, in front of the barrier that publishes the buffer.  (Nothing else in the kernel uses m0.)
 __device__ __forceinline__ void lds_load(u4 r, unsigned off, unsigned to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory");
 }
 
-// One operand's way into LDS: a tile of R rows x 64 k by W waves.
+// Permutation of the 32-byte slots of row k: half a wave of ds_read_b64_tr_b16 reads rows 8 g .. + 4 of two neighbouring g,
+// which have to lie in eight different slots (mod 8: 256 bytes, all banks once)
+__device__ __forceinline__ int slot_of(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+
+// One operand's way into LDS: a tile of R rows x 32 k by W waves.
 template <int R, int W, bool ROWS>
 struct Loader {
     static constexpr int kLoads = R * kBK * 2 / 1024 / W;      // 1024-byte loads per wave
@@ -53,51 +62,45 @@ struct Loader {
             if (ROWS) {
                 const int b = j * 1024 + lane * 16;
                 const int kk = b / (R * 2), p = (b >> 4) & (kPieces - 1);
-                const int piece = p ^ (2 * (kk & (kPieces / 2 - 1)));
+                const int piece = p ^ (2 * slot_of(kk));
                 k[q] = kk;
                 off[q] = piece * 8 < rows_left ? (unsigned)(kk * ld * 2 + piece * 16) : kOutside;
             } else {
-                const int row = j * 8 + (lane >> 3), piece = (lane & 7) ^ (row & 7);
+                const int row = j * 16 + (lane >> 2), piece = (lane & 3) ^ ((row >> 1) & 3);
                 k[q] = piece * 8;
                 off[q] = row < rows_left ? (unsigned)(row * ld * 2 + piece * 16) : kOutside;
             }
         }
     }
-    // base: the tile's first row at this step's first k; k_left: valid k indices from there
-    __device__ __forceinline__ void load(const char *base, int k_left, char *lds, int wave) const {
+    // base: the tile's first row at this step's first k; k_left: valid k indices from there (none: all lanes get zeros)
+    __device__ __forceinline__ void load(const char *base, int k_left, unsigned lds, int wave) const {
         const u4 r = {(unsigned)(uintptr_t)base, (unsigned)((uintptr_t)base >> 32) & 0xffff, 0x7fffffffu, 0x00020000u};
-        const unsigned to = (unsigned)(uintptr_t)(lds_ptr)(lds + wave * kLoads * 1024);
 #pragma unroll
-        for (int q = 0; q < kLoads; ++q) lds_load(r, k[q] < k_left ? off[q] : kOutside, to + q * 1024);
+        for (int q = 0; q < kLoads; ++q) lds_load(r, k[q] < k_left ? off[q] : kOutside, lds + (wave * kLoads + q) * 1024);
     }
 };
 
-// Fragments of a wave: F blocks of 16 rows from row `first` on, 32 k each (half s of the step)
+// Fragments of a wave: F blocks of 16 rows from row `first` on
 template <int R, int F, bool ROWS>
 struct Reader {
-    int at[ROWS ? F : 2];
+    int at[ROWS ? F : 1];
     __device__ __forceinline__ void init(int first, int lane) {
         const int i = lane & 15, g = lane >> 4;
         if (ROWS) {
-            constexpr int slots = R / 16;
             const int kk = 8 * g + (i >> 2);
 #pragma unroll
-            for (int f = 0; f < F; ++f) at[f] = kk * R * 2 + (((first / 16 + f) ^ (kk & (slots - 1))) * 32) + (i & 3) * 8;
+            for (int f = 0; f < F; ++f) at[f] = kk * R * 2 + (((first / 16 + f) ^ slot_of(kk)) * 32) + (i & 3) * 8;
         } else {
-            at[0] = (first + i) * 128 + ((g ^ (i & 7)) * 16);
-            at[1] = (first + i) * 128 + (((g + 4) ^ (i & 7)) * 16);
+            at[0] = (first + i) * 64 + ((g ^ ((i >> 1) & 3)) * 16);
         }
     }
-    __device__ __forceinline__ s8 read(const char *lds, int f, int s) const {
-        if (ROWS) {
-            // k + 4 flips bit 2 of the slot permutation: the same place as block f ^ 4 four rows on (F >= 8), or computed
-            const char *p = lds + at[f] + s * 32 * R * 2;
-            const char *p2 = lds + (at[f] ^ 128) + s * 32 * R * 2 + 4 * R * 2;
-            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
-            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p2);
+    __device__ __forceinline__ s8 read(const char *lds, int f) const {
+        if (ROWS) {                                            // (k + 4 has the same permutation)
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at[f]));
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at[f] + 4 * R * 2));
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
-        return *(const s8 *)(lds + at[s] + f * 2048);
+        return *(const s8 *)(lds + at[0] + f * 1024);
     }
 };
 
@@ -107,8 +110,8 @@ __device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1,
 template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB>
 __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : WM * WN / 2) void tile_kernel(Product P) {
     constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, kA = BM * kBK * 2, kB = BN * kBK * 2;
-    static_assert(FN == 4 && FM % 4 == 0 && W * 16384 <= 2 * (kA + kB), "the epilogue takes 64 x 64 of a wave at a time");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (kA + kB)];
+    static_assert(FN == 4 && FM % 4 == 0 && W * 16384 <= kRing * (kA + kB), "the epilogue takes 64 x 64 of a wave at a time");
+    __shared__ __attribute__((aligned(1024))) char lds[kRing * (kA + kB)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // tiles in groups of eight tile rows, each XCD a contiguous run of them: neighbours share operands in one L2
     const unsigned tm = (unsigned)((P.M + BM - 1) / BM), tn = (unsigned)((P.N + BN - 1) / BN), total = tm * tn;
@@ -128,43 +131,68 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : WM * WN / 2)
     rb.init(wn, lane);
 
     const long per = (P.K + kBK - 1) / kBK;            // steps of one pass over k
-    const long first = (long)blockIdx.y * P.kchunk, steps = per * P.passes;
-    const long last = first + P.kchunk < steps ? first + P.kchunk : steps;
-    const char *A = (const char *)P.a + (TA ? m0 : m0 * P.lda) * 2, *B = (const char *)P.b + (TB ? n0 : n0 * P.ldb) * 2;
+    const long first = (long)blockIdx.y * P.kchunk, all = per * P.passes;
+    const int steps = (int)((first + P.kchunk < all ? first + P.kchunk : all) - first);
+    const char *A0 = (const char *)P.a + (TA ? m0 : m0 * P.lda) * 2, *B0 = (const char *)P.b + (TB ? n0 : n0 * P.ldb) * 2;
     const long stepa = (TA ? P.lda : 1) * kBK * 2, stepb = (TB ? P.ldb : 1) * kBK * 2;
 
-    auto issue = [&](long step, char *to) {
-        const long pass = P.passes == 1 ? 0 : step / per, k = P.passes == 1 ? step : step - pass * per;
-        const char *a = A + k * stepa, *b = B + k * stepb;
-        if (P.passes > 1) {
+    // the next step to load
+    int pass = (int)(first / per), ahead = 0;
+    long kstep = first - pass * per;
+    const unsigned base = (unsigned)(uintptr_t)(lds_ptr)lds;
+    unsigned to_at = 0, cur_at = 0;
+    auto issue = [&]() {
+        const char *a = A0 + kstep * stepa, *b = B0 + kstep * stepb;
+        if (P.passes > 1 && pass < 6) {
             a += kPlaneA[pass] * P.plane_a * 2;
             b += kPlaneB[pass] * P.plane_b * 2;
         }
-        const long left = P.K - k * kBK;
-        la.load(a, left < kBK ? (int)left : kBK, to, wave);
-        lb.load(b, left < kBK ? (int)left : kBK, to + kA, wave);
+        const long k_left = P.K - kstep * kBK;
+        const int left = ahead >= steps ? 0 : k_left < kBK ? (int)k_left : kBK;
+        const unsigned to = base + to_at;
+        to_at = to_at == (kRing - 1) * (kA + kB) ? 0 : to_at + kA + kB;
+        la.load(a, left, to, wave);
+        lb.load(b, left, to + kA, wave);
+        ++ahead;
+        if (++kstep == per) kstep = 0, ++pass;
     };
 
+    // Loads return in order: with all but the first of the steps ahead outstanding, that one has arrived.
+    constexpr int kFly = (kRing - 2) * (Loader<BM, W, TA>::kLoads + Loader<BN, W, TB>::kLoads);
+    static_assert(kFly < 16, "vmcnt's low field");
     f4 acc[FN][FM] = {};
-    if (first < last) issue(first, lds);
-    for (long step = first; step < last; ++step) {
-        char *cur = lds + (int)((step - first) & 1) * (kA + kB), *nxt = lds + (int)((step - first + 1) & 1) * (kA + kB);
-        __builtin_amdgcn_s_waitcnt(0x0f70);            // vmcnt(0): this wave's part of the step has arrived
-        __syncthreads();                               // and every wave's; nobody reads the other buffer any more
-        if (step + 1 < last) issue(step + 1, nxt);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            s8 fa[FM], fb[FN];
+    for (int i = 0; i < kRing - 1; ++i) issue();
+    __builtin_amdgcn_s_waitcnt(0x0f70 | kFly);
+    __builtin_amdgcn_s_barrier();
+    if (W == 8 && wave >= 4) __builtin_amdgcn_s_barrier();
+    for (int step = 0; step < steps; ++step) {
+        // Reads of this step's buffer; loads of the third step from here into the buffer that every wave left a barrier ago.
+        const char *cur = lds + cur_at;
+        cur_at = cur_at == (kRing - 1) * (kA + kB) ? 0 : cur_at + kA + kB;
+        s8 fa[FM], fb[FN];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = ra.read(cur, i, s);
+        for (int j = 0; j < FN; ++j) fb[j] = rb.read(cur + kA, j);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = rb.read(cur + kA, j, s);
+        for (int i = 0; i < FM; ++i) fa[i] = ra.read(cur, i);
+        issue();
+        // the fragments are here, and of the ring the next step's buffer (this wave's part: the barrier makes it everyone's)
+        __builtin_amdgcn_s_waitcnt(0x0070 | kFly);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int i = 0; i < FM; ++i) acc[j][i] = mfma<MT>(fb[j], fa[i], acc[j][i]);
-        }
+            for (int i = 0; i < FM; ++i) acc[j][i] = mfma<MT>(fb[j], fa[i], acc[j][i]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (W == 8) __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     }
+    if (W == 8 && wave < 4) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // the zeros of the steps past the end have arrived too
 
     // The sums leave through LDS, 64 x 64 of a wave at a time (16 KB of its own): the epilogue's code then exists once, and
     // eight lanes write 128 neighbouring bytes (16-bit) of a row.  16-byte pieces of a row are permuted by ^ row & 15.

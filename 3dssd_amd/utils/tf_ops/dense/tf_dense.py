@@ -20,16 +20,24 @@ from ... import _native as N
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
-_MAX_CHANNELS = (1 << 31) - 1
+_FAR = 1 << 24                        # rows further apart than this are copied together; longer ones are refused
 
 
 def _operand(t, name, dtype=None):
+    """Raises unless t is a tensor the kernels can read."""
     T.require(isinstance(t, torch.Tensor), "%s must be a torch.Tensor" % name)
     T.require(t.is_cuda, "%s must live on the GPU (the HIP path has no CPU fallback)" % name)
     T._on_current_device(t, name)
     T.require(t.dtype in TYPES, "%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
     T.require(dtype is None or t.dtype == dtype, "%s is %s but inputs are %s" % (name, t.dtype, dtype))
-    return t
+
+
+def _beside(t, name, inputs, *dtypes):
+    """Raises unless t is a tensor beside inputs, of its type (or one of dtypes)."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == inputs.get_device() and
+            (t.dtype == inputs.dtype or t.dtype in dtypes)):
+        _operand(t, name, None if dtypes else inputs.dtype)
+        raise ValueError("%s must be float32 or of the inputs' type" % name)
 
 
 def _rows(t, cols):
@@ -37,9 +45,11 @@ def _rows(t, cols):
     it, a copy otherwise."""
     m = t if t.dim() == 2 else t.reshape(-1, cols)
     rows = m.shape[0]
-    if cols > 1 and m.stride(1) != 1 or rows > 1 and m.stride(0) < cols:
+    ld, step = m.stride()
+    if (step != 1 and cols > 1) or ((ld < cols or ld >= _FAR) and rows > 1):
         m = m.contiguous()
-    return m, m.data_ptr(), (m.stride(0) if rows > 1 else cols)
+        ld = cols
+    return m, m.data_ptr(), (ld if rows > 1 else cols)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -57,19 +67,31 @@ def _backward_ws(*args):
 
 
 def _layer(op, inputs, weights, biases, activation):
-    _operand(inputs, "inputs")
-    dt = inputs.dtype
-    _operand(weights, "weights", dt)
-    T.require(activation in ACTIVATIONS, "%s knows the activations %s, not %r" % (op, sorted(a for a in ACTIVATIONS if a), activation))
-    T.require(weights.dim() == 2, "%s expects (cin,cout) weights shape" % op)
-    T.require(inputs.dim() >= 1 and inputs.shape[-1] == weights.shape[0], "%s expects (...,cin) inputs shape" % op)
+    """Checks what both functions take; (type, cin, cout, device).  One pass over the conditions in the ordinary case: the
+    messages are only made where one of them does not hold."""
+    if not (isinstance(inputs, torch.Tensor) and isinstance(weights, torch.Tensor) and inputs.is_cuda and
+            inputs.get_device() == weights.get_device() == torch.cuda.current_device() and
+            inputs.dtype == weights.dtype and inputs.dtype in TYPES):
+        _operand(inputs, "inputs")
+        _operand(weights, "weights", inputs.dtype)
+    if activation not in ACTIVATIONS:
+        raise ValueError("%s knows the activations %s, not %r" % (op, sorted(a for a in ACTIVATIONS if a), activation))
+    if weights.dim() != 2:
+        raise ValueError("%s expects (cin,cout) weights shape" % op)
     cin, cout = weights.shape
-    T.require(max(cin, cout) <= _MAX_CHANNELS, "%s expects fewer than 2**31 channels" % op)
+    if inputs.dim() == 0 or inputs.shape[-1] != cin:
+        raise ValueError("%s expects (...,cin) inputs shape" % op)
+    if max(cin, cout) >= _FAR:
+        raise ValueError("%s expects fewer than 2**24 channels" % op)
     if biases is not None:
-        _operand(biases, "biases")
-        T.require(biases.dtype in (dt, torch.float32), "biases must be float32 or of the inputs' type")
-        T.require(tuple(biases.shape) == (cout,), "%s expects (cout) biases shape" % op)
-    return dt, cin, cout
+        _beside(biases, "biases", inputs, torch.float32)
+        if biases.shape != (cout,):
+            raise ValueError("%s expects (cout) biases shape" % op)
+    return inputs.dtype, cin, cout
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _aligned(ptr, ld, itemsize):
@@ -87,10 +109,10 @@ def dense(inputs, weights, biases=None, activation=None, residual=None, return_p
     dt, cin, cout = _layer("Dense", inputs, weights, biases, activation)
     shape = inputs.shape[:-1] + (cout,)
     if residual is not None:
-        _operand(residual, "residual", dt)
+        _beside(residual, "residual", inputs)
         T.require(residual.shape == shape, "Dense expects (...,cout) residual shape")
-    out = torch.empty(shape, dtype=dt, device=inputs.device)
-    pre = torch.empty_like(out) if return_preact else None
+    out = inputs.new_empty(shape)
+    pre = inputs.new_empty(shape) if return_preact else None
     rows = out.numel() // cout if cout else 0
     if rows:
         x, xp, ldx = _rows(inputs, cin)
@@ -99,11 +121,11 @@ def dense(inputs, weights, biases=None, activation=None, residual=None, return_p
         b = None if biases is None else biases.contiguous()
         code, e = TYPES[dt], dt.itemsize
         need = _forward_ws(code, rows, cin, cout, _aligned(xp, ldx, e) + 2 * _aligned(wp, ldw, e))
-        ws = torch.empty(need, dtype=torch.uint8, device=inputs.device) if need else None
+        ws = inputs.new_empty(need, dtype=torch.uint8) if need else None
         N.check(N.lib().sa_dense_forward(code, rows, cin, cout, xp, ldx, wp, ldw, None if b is None else b.data_ptr(),
                                          int(b is not None and b.dtype == torch.float32), rp, ldr, ACTIVATIONS[activation],
                                          out.data_ptr(), None if pre is None else pre.data_ptr(),
-                                         None if ws is None else ws.data_ptr(), need, N.current_stream()), "dense")
+                                         None if ws is None else ws.data_ptr(), need, _stream(inputs.get_device())), "dense")
     return (out, pre) if return_preact else out
 
 
@@ -117,19 +139,18 @@ def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=N
     bias gradient sums it unrounded.  Sums run in fp32 in a fixed order: the same call gives the same bits."""
     dt, cin, cout = _layer("DenseGrad", inputs, weights, biases, activation)
     shape = inputs.shape[:-1] + (cout,)
-    _operand(grad_out, "grad_out", dt)
+    _beside(grad_out, "grad_out", inputs)
     T.require(grad_out.shape == shape, "DenseGrad expects (...,cout) grad_out shape")
     if activation is None:
         preact = None
     else:
         T.require(preact is not None, "DenseGrad needs preact where there is an activation")
-        _operand(preact, "preact", dt)
+        _beside(preact, "preact", inputs)
         T.require(preact.shape == shape, "DenseGrad expects (...,cout) preact shape")
     T.require(len(needs) == 2, "needs: (inputs, weights)")
-    dev = inputs.device
-    dx = torch.empty(inputs.shape, dtype=dt, device=dev) if needs[0] else None
-    dw = torch.empty((cin, cout), dtype=dt, device=dev) if needs[1] else None
-    db = torch.empty((cout,), dtype=biases.dtype, device=dev) if biases is not None else None
+    dx = inputs.new_empty(inputs.shape) if needs[0] else None
+    dw = inputs.new_empty((cin, cout)) if needs[1] else None
+    db = biases.new_empty((cout,)) if biases is not None else None
     rows = 1
     for d in inputs.shape[:-1]:
         rows *= d
@@ -143,9 +164,9 @@ def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=N
     if want:
         aligned = sum(1 << i for i, (p, ld) in enumerate(((xp, ldx), (wp, ldw), (gp, ldg))) if p and _aligned(p, ld, e))
         need = _backward_ws(code, rows, cin, cout, act, want, aligned)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        ws = inputs.new_empty(need, dtype=torch.uint8) if need else None
         N.check(N.lib().sa_dense_backward(code, rows, cin, cout, xp, ldx, wp, ldw, gp, ldg, zp, ldz, act,
                                           dx.data_ptr() if want & 1 else None, dw.data_ptr() if want & 2 else None,
                                           db.data_ptr() if want & 4 else None, int(db is not None and db.dtype == torch.float32),
-                                          None if ws is None else ws.data_ptr(), need, N.current_stream()), "dense_grad")
+                                          None if ws is None else ws.data_ptr(), need, _stream(inputs.get_device())), "dense_grad")
     return dx, dw, db

@@ -7,6 +7,7 @@ the argument order and the results follow the TensorFlow functions it calls.  Th
 """
 import bisect
 import ctypes
+import functools
 
 import torch
 
@@ -35,39 +36,50 @@ def _dense_memory(t):
     return True
 
 
+def _gather(t_list, op):
+    """The tensors of the list (None entries dropped) and the device they are on, checked."""
+    T.require(isinstance(t_list, (list, tuple)), "%s expects a list of tensors" % op)
+    ts = [t for t in t_list if t is not None]
+    device = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
+    if device < 0 or not all([isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype in TYPES for t in ts]):
+        for i, t in enumerate(t_list):                 # say which
+            if t is not None:
+                _check(t, "t_list[%d]" % i)
+        raise ValueError("%s needs a GPU (the HIP path has no CPU fallback)" % op)
+    return ts, device
+
+
 def _arrays(ts):
     k = len(ts)
     return ((ctypes.c_void_p * k)(*[t.data_ptr() for t in ts]), (ctypes.c_long * k)(*[t.numel() for t in ts]),
             (ctypes.c_int * k)(*[TYPES[t.dtype] for t in ts]))
 
 
-def _gather(t_list, op):
-    T.require(isinstance(t_list, (list, tuple)), "%s expects a list of tensors" % op)
-    ts = []
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for i, t in enumerate(t_list):
-        if t is None:
-            continue
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == device and t.dtype in TYPES):
-            _check(t, "t_list[%d]" % i)
-        ts.append(t)
-    return ts
-
-
-def _scratch(count):
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(count):
     n = ctypes.c_ulong()
     N.check(N.lib().sa_global_norm_ws(count, ctypes.byref(n)), "global_norm")
-    return torch.empty(n.value, dtype=torch.uint8, device="cuda"), n.value
+    return n.value
+
+
+def _scalar_and_scratch(count, device):
+    """The norm's fp32 scalar and the scratch of a call on `count` tensors."""
+    size = _ws_bytes(count)
+    return (torch.empty((), dtype=torch.float32, device=device), torch.empty(size, dtype=torch.uint8, device=device), size)
+
+
+def _packed(ts):
+    return [t if t.is_contiguous() or _dense_memory(t) else t.contiguous() for t in ts]
 
 
 def global_norm(t_list):
     """sqrt of the sum of all squares, a float32 scalar tensor on the GPU.  Sums are held in 64 bits, in a fixed order."""
-    ts = [t if _dense_memory(t) else t.contiguous() for t in _gather(t_list, "GlobalNorm")]
-    T.require(torch.cuda.is_available(), "GlobalNorm needs a GPU (the HIP path has no CPU fallback)")
-    norm = torch.empty((), dtype=torch.float32, device="cuda")
+    ts, device = _gather(t_list, "GlobalNorm")
+    ts = _packed(ts)
     p, n, kinds = _arrays(ts)
-    ws, size = _scratch(len(ts))
-    N.check(N.lib().sa_global_norm(len(ts), p, n, kinds, norm.data_ptr(), ws.data_ptr(), size, N.current_stream()), "global_norm")
+    norm, ws, size = _scalar_and_scratch(len(ts), device)
+    N.check(N.lib().sa_global_norm(len(ts), p, n, kinds, norm.data_ptr(), ws.data_ptr(), size,
+                                   torch._C._cuda_getCurrentRawStream(device)), "global_norm")
     return norm
 
 
@@ -86,22 +98,19 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
     out: None for new tensors, t_list itself to clip in place (nothing is written where the norm is within bounds), or a
     list of tensors of the same shapes and types.  Results must not overlap one another, nor any gradient but their own,
     which they may only share whole; each must be dense in memory, in its gradient's order of dimensions."""
-    ts = _gather(t_list, "ClipByGlobalNorm")
     clip = float(clip_norm)
     T.require(clip > 0, "ClipByGlobalNorm expects a positive clip_norm")
-    T.require(torch.cuda.is_available(), "ClipByGlobalNorm needs a GPU (the HIP path has no CPU fallback)")
+    ts, device = _gather(t_list, "ClipByGlobalNorm")
     if use_norm is not None:
         _check(use_norm, "use_norm")
         T.require(use_norm.dtype == torch.float32 and use_norm.numel() == 1, "ClipByGlobalNorm expects a float32 scalar use_norm")
     if out is None:
-        ts = [t if _dense_memory(t) else t.contiguous() for t in ts]
+        ts = _packed(ts)
         results = [torch.empty_like(t) for t in ts]
-        given = None
     else:
         T.require(isinstance(out, (list, tuple)) and len(out) == len(t_list), "ClipByGlobalNorm expects as many out tensors as gradients")
         in_place = out is t_list
-        given = [o for o, t in zip(out, t_list) if t is not None]
-        results = given
+        results = [o for o, t in zip(out, t_list) if t is not None]
         for i, (t, o) in enumerate(zip(ts, results)):
             if not in_place:
                 _check(o, "out[%d]" % i)
@@ -113,18 +122,18 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
         moved = [] if in_place else [t for t, o in zip(ts, results) if t.data_ptr() != o.data_ptr()]
         T.require(not _overlap_between(results, moved), "ClipByGlobalNorm cannot write over another gradient")
         T.require(use_norm is None or not _overlap_between(results, [use_norm]), "ClipByGlobalNorm cannot write over use_norm")
-    k = len(ts)
     p, n, kinds = _arrays(ts)
-    o = (ctypes.c_void_p * k)(*[t.data_ptr() for t in results])
+    o = (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in results])
     if use_norm is None:
-        norm = torch.empty((), dtype=torch.float32, device="cuda")
-        ws, size = _scratch(k)
-        N.check(N.lib().sa_clip_by_global_norm(k, p, o, n, kinds, clip, None, norm.data_ptr(), ws.data_ptr(), size,
-                                               N.current_stream()), "clip_by_global_norm")
+        norm, ws, size = _scalar_and_scratch(len(ts), device)
+        given, to, scratch = None, norm.data_ptr(), ws.data_ptr()
     else:
-        norm = use_norm
-        N.check(N.lib().sa_clip_by_global_norm(k, p, o, n, kinds, clip, norm.data_ptr(), None, None, 0, N.current_stream()),
-                "clip_by_global_norm")
+        norm, size = use_norm, 0
+        given, to, scratch = norm.data_ptr(), None, None
+    N.check(N.lib().sa_clip_by_global_norm(len(ts), p, o, n, kinds, clip, given, to, scratch, size,
+                                           torch._C._cuda_getCurrentRawStream(device)), "clip_by_global_norm")
+    if len(results) == len(t_list):
+        return results, norm
     it = iter(results)
     return [None if t is None else next(it) for t in t_list], norm
 

@@ -138,6 +138,7 @@ def test_the_c_entries_refuse_what_they_cannot_compute():
     n = ctypes.c_ulong()
     by = ctypes.byref(n)
     assert lib.sa_dense_forward_ws(3, 1, 1, 1, 0, by) == -1 and lib.sa_dense_forward_ws(0, -1, 1, 1, 0, by) == -1
+    assert lib.sa_dense_forward_ws(0, 1, 1 << 24, 1, 0, by) == -1
     assert lib.sa_dense_forward_ws(0, 1, 1, 1, 0, None) == -1
     assert lib.sa_dense_backward_ws(0, 1, 1, 1, 9, 7, 0, by) == -1 and lib.sa_dense_backward_ws(0, 1, 1, 1, 0, 8, 0, by) == -1
     p = 1 << 20                                        # an address that is never dereferenced: every call below is refused
@@ -148,15 +149,16 @@ def test_the_c_entries_refuse_what_they_cannot_compute():
     assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
     assert fwd(ldx=7) == -1 and fwd(ldw=7) == -1 and fwd(res=p, ldr=7) == -1
     assert fwd(rows=0) == 0 and fwd(cout=0) == 0       # nothing to compute
-    assert lib.sa_dense_forward_ws(1, 4, 4096, 8, 3, by) == 0 and n.value > 0
-    assert fwd(cin=4096, ldx=4096) == -1               # scratch missing
-    assert fwd(cin=4096, ldx=4096, ws=p, wsb=n.value - 1) == -1
+    assert lib.sa_dense_forward_ws(1, 400, 4096, 8, 3, by) == 0 and n.value > 0
+    assert fwd(rows=400, cin=4096, ldx=4096) == -1     # scratch missing
+    assert fwd(rows=400, cin=4096, ldx=4096, ws=p, wsb=n.value - 1) == -1
+    assert fwd(ldx=1 << 24) == -3 and fwd(ldw=1 << 24) == -3   # offsets inside a tile would not fit
     bwd = lambda **k: lib.sa_dense_backward(*[k.get(a, d) for a, d in (   # noqa: E731
         ("dtype", 1), ("rows", 4), ("cin", 8), ("cout", 8), ("x", p), ("ldx", 8), ("w", p), ("ldw", 8), ("g", p), ("ldg", 8),
         ("z", p), ("ldz", 8), ("act", 1), ("dx", p), ("dw", p), ("db", p), ("df", 0), ("ws", None), ("wsb", 0), ("stream", None))])
     assert bwd() == -1                                 # scratch missing
     assert bwd(g=None) == -1 and bwd(z=None) == -1 and bwd(x=None) == -1 and bwd(w=None) == -1 and bwd(ldg=7) == -1
-    assert bwd(dx=None, dw=None, db=None) == 0
+    assert bwd(dx=None, dw=None, db=None) == 0 and bwd(ldg=1 << 24) == -3 and bwd(ldw=1 << 24) == -3
 
 
 # --------------------------------------------------------------------------------------------------------- GPU: values
