@@ -242,7 +242,7 @@ int launch_jobs(int type, Jobs &J, int n, hipStream_t s) {
 }
 
 // A product and its k pieces.  Tiles: 256 x 256 where they fill the chip, else 128 x 128, two workgroups per CU, at least
-// eight steps each.  Small: blocks of 32 x 32, two workgroups per CU, at least 2048 k each (sixteen waves, four steps).
+// four steps each.  Small: blocks of 32 x 32, two workgroups per CU, at least 2048 k each (sixteen waves, four steps).
 struct Plan {
     Product P;
     bool ta, tb;
@@ -257,7 +257,7 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     P.passes = type == kF32 && tiles ? 6 : 1;
     auto count = [&](long e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
     L.edge = !tiles ? 0 : count(256) >= 192 ? 256 : 128;
-    const long steps = (K + 31) / 32 * P.passes, least = tiles ? 8 : 64;
+    const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes, least = tiles ? 4 : 64;
     const long blocks = count(tiles ? L.edge : 32), slots = L.edge == 256 ? 256 : 512;
     long s = slots / blocks;
     if (s > steps / least) s = steps / least;

@@ -9,7 +9,7 @@ constexpr long kMaxTileLd = 1L << 21, kMaxLd = 1L << 24;
 
 // D = A B^T on tiles of edge x edge (128 or 256) of 16-bit operands with 16-byte aligned bases and rows, and whole 16-byte
 // pieces along the contiguous index.  type: kBF16 / kF16 of the operands; out_type: that, or kF32.  P.kchunk counts steps of
-// 32 k over all passes.  ta and not tb does not occur.
+// 64 k over all passes.  ta and not tb does not occur.
 int launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
 
 // Any product; P.kchunk counts k indices (a multiple of 32).
