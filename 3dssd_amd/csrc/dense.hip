@@ -8,18 +8,15 @@ using namespace dense;
 
 namespace {
 
-template <class T> struct alignas(16) Eight { T x[8]; };
+template <class T> using Eight = Pack<T, 8>;
 
 // Columns c .. c + 8 of a row; zeros behind the last column.
 template <class T>
-__device__ __forceinline__ Eight<T> fetch(const T *row, int vec, int c, int cols) {
+__device__ __forceinline__ Eight<T> fetch(const T *row, int c, int cols) {
+    if (c + 8 <= cols) return load_pack<T, 8>(row + c);
     Eight<T> v;
-    if (vec && c + 8 <= cols) {
-        v = *(const Eight<T> *)(row + c);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.x[i] = c + i < cols ? row[c + i] : T{};
-    }
+    for (int i = 0; i < 8; ++i) v.x[i] = c + i < cols ? row[c + i] : T{};
     return v;
 }
 
@@ -55,7 +52,6 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
 struct Job {
     const void *g, *z;    // z null: no activation
     long ldg, ldz;
-    int vec;              // g and z: 16-byte aligned bases and rows
     int act;
     long rows;
     int cols;
@@ -100,8 +96,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
 #pragma unroll
         for (int u = 0; u < kRows; ++u)
             if (r + 8 * u < r1) {
-                g[u] = fetch((const T *)S.g + (r + 8 * u) * S.ldg, S.vec, c0, S.cols);
-                if (S.z) z[u] = fetch((const T *)S.z + (r + 8 * u) * S.ldz, S.vec, c0, S.cols);
+                g[u] = fetch((const T *)S.g + (r + 8 * u) * S.ldg, c0, S.cols);
+                if (S.z) z[u] = fetch((const T *)S.z + (r + 8 * u) * S.ldz, c0, S.cols);
             }
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
@@ -129,12 +125,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
                         for (int p = 0; p < 3; ++p) o[p].x[i].u = h[p];
                     }
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) *(Eight<bf16_t> *)((bf16_t *)S.dst + p * S.plane + at) = o[p];
+                    for (int p = 0; p < 3; ++p) store_pack<bf16_t, 8>((bf16_t *)S.dst + p * S.plane + at, o[p]);
                 } else {
                     Eight<T> o;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
-                    *(Eight<T> *)((T *)S.dst + at) = o;
+                    store_pack<T, 8>((T *)S.dst + at, o);
                 }
             }
 #pragma unroll
@@ -221,7 +217,7 @@ long strip_of(long rows, int cols) {
 }
 void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
     Job j{};
-    j.g = m.p; j.ldg = m.ld; j.vec = m.vec; j.rows = m.rows; j.cols = m.cols;
+    j.g = m.p; j.ldg = m.ld; j.rows = m.rows; j.cols = m.cols;
     j.ldd = round_up(m.cols, 8);
     j.plane = type == kF32 ? m.rows * j.ldd : 0;
     j.dst = ws.take((unsigned long)m.rows * j.ldd * 2 * (type == kF32 ? 3 : 1));
@@ -317,7 +313,6 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     const bool products = want & (kWantX | kWantW);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
-    j.vec = g.vec && (act == kNone || z.vec);
     j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
     j.strip = strip_of(rows, cout);
     Matrix d = g;
@@ -366,8 +361,7 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
                  Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)});
     if (s.used > ws_bytes || (s.used && !ws)) return SA_ERR_INVALID;
     Epilogue &e = f.plan.P.e;
-    e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act, 0};
-    e.vec = cout % 8 == 0 && aligned(y, cout, dtype) && (!pre || aligned(pre, cout, dtype)) && (!res || aligned(res, ldr, dtype));
+    e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act};
     const int rc = launch_jobs(dtype, f.jobs, f.njobs, (hipStream_t)stream);
     return rc ? rc : launch_plan(dtype, f.plan, (hipStream_t)stream);
 }
@@ -413,11 +407,11 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
         SA_CHECK_LAUNCH();
     }
     if (want & kWantX) {
-        b.dx.P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cin % 8 == 0 && aligned(dx, cin, dtype)};
+        b.dx.P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
         if ((rc = launch_plan(dtype, b.dx, st))) return rc;
     }
     if (want & kWantW) {
-        b.dw.P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone, cout % 8 == 0 && aligned(dw, cout, dtype)};
+        b.dw.P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
         if ((rc = launch_plan(dtype, b.dw, st))) return rc;
     }
     return SA_OK;
