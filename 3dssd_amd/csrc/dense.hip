@@ -1,8 +1,8 @@
 // The dense layer on plain weights: y = act(x W + b) + residual in fp32, bf16 or fp16, and its gradient
 // (dense_common.h has the formulas).  This file: the pass in front of the products that need one, the join of split sums,
-// the choice of kernel, and the C ABI.  The products are in dense_tile.hip (large) and dense_small.hip.
+// the choice of kernel, and the C ABI.  The products are in dense_products.hip (large) and dense_small.hip.
 #include "dense_common.h"
-#include "dense_tile.h"
+#include "dense_products.h"
 
 using namespace dense;
 
@@ -107,11 +107,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
             for (int i = 0; i < 8; ++i) d[i] = to_f32<T>(g[u].x[i]);
             if (S.z) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float zi = to_f32<T>(z[u].x[i]);
-                    if (S.act == kRelu) d[i] = zi > 0.0f ? d[i] : (zi != zi ? zi : 0.0f);
-                    else d[i] = c0 + i < S.cols ? d[i] * act_slope(zi, S.act) : 0.0f;
-                }
+                for (int i = 0; i < 8; ++i) d[i] = times_slope(d[i], to_f32<T>(z[u].x[i]), S.act);
             }
             if (S.dst) {
                 const long at = (r + 8 * u) * S.ldd + c0;
@@ -238,13 +234,15 @@ int launch_jobs(int type, Jobs &J, int n, hipStream_t s) {
 }
 
 // A product and its k pieces.  Tiles: 256 x 256 where they fill the chip, else 128 x 128, two workgroups per CU, at least
-// four steps each.  Small: blocks of 32 x 32, two workgroups per CU, at least 2048 k each (sixteen waves, four steps).
+// four steps each.  Small: blocks of 32 x 32 up to one per CU, and pieces long enough to be worth the join's launch (4 us):
+// `least` steps of 32 k.
 struct Plan {
     Product P;
     bool ta, tb;
-    int edge;             // 0: launch_small
+    int edge;             // of the tiles; 0: a small product
 };
-void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K) {
+void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K,
+          long least) {
     Product &P = L.P;
     L.ta = ta; L.tb = tb;
     P.M = M; P.N = N; P.K = K;
@@ -253,8 +251,9 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     P.passes = type == kF32 && tiles ? 6 : 1;
     auto count = [&](long e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
     L.edge = !tiles ? 0 : count(256) >= 192 ? 256 : 128;
-    const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes, least = tiles ? 4 : 64;
-    const long blocks = count(tiles ? L.edge : 32), slots = L.edge == 256 ? 256 : 512;
+    const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
+    if (tiles) least = 4;
+    const long blocks = count(tiles ? L.edge : 32), slots = L.edge == 128 ? 512 : 256;
     long s = slots / blocks;
     if (s > steps / least) s = steps / least;
     if (s < 1) s = 1;
@@ -266,20 +265,27 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * M * round_up(N, 4) * 4) : nullptr;
 }
 
-template <class T>
-int launch_plan(const Plan &L, hipStream_t s) {
-    const Product &P = L.P;
-    const int type = sizeof(T) == 4 ? kF32 : __is_same(T, bf16_t) ? kBF16 : kF16;
-    const int rc = L.edge ? launch_tiles(L.edge, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, P, s)
-                          : launch_small(type, L.ta, L.tb, P, s);
-    if (rc || P.splits == 1) return rc;
-    const long blocks = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, P);
+int launch_join(int type, const Product &P, hipStream_t s) {
+    if (P.splits == 1) return SA_OK;
+    const long n = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
+    const dim3 blocks((unsigned)(n < 8192 ? n : 8192));
+    if (type == kF32) hipLaunchKernelGGL((join_kernel<float>), blocks, dim3(256), 0, s, P);
+    else if (type == kBF16) hipLaunchKernelGGL((join_kernel<bf16_t>), blocks, dim3(256), 0, s, P);
+    else hipLaunchKernelGGL((join_kernel<f16_t>), blocks, dim3(256), 0, s, P);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
-int launch_plan(int type, const Plan &L, hipStream_t s) {
-    return type == kF32 ? launch_plan<float>(L, s) : type == kBF16 ? launch_plan<bf16_t>(L, s) : launch_plan<f16_t>(L, s);
+int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
+    const int rc = launch_tiles(L.edge, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
+    return rc ? rc : launch_join(type, L.P, s);
+}
+int launch_sums(int type, const float *sums, int strips, int cols, void *out, int out_f32, hipStream_t s) {
+    const dim3 grid((cols + 63) / 64);
+    if (out_f32 || type == kF32) hipLaunchKernelGGL((sum_strips_kernel<float>), grid, dim3(256), 0, s, sums, strips, cols, (float *)out);
+    else if (type == kBF16) hipLaunchKernelGGL((sum_strips_kernel<bf16_t>), grid, dim3(256), 0, s, sums, strips, cols, (bf16_t *)out);
+    else hipLaunchKernelGGL((sum_strips_kernel<f16_t>), grid, dim3(256), 0, s, sums, strips, cols, (f16_t *)out);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
 }
 
 struct Forward {
@@ -294,44 +300,60 @@ void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cou
         if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
     }
-    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin);
+    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin, rows <= 32 ? 128 : 64);
 }
 
 struct Backward {
     Jobs jobs;
     int njobs;
+    bool tiles;
     Plan dx, dw;
-    float *sums;
+    float *sums;          // the bias gradient's partial sums: of the jobs' strips, or of dW's pieces
     int strips;
+    bool bias_in_dw;
 };
 constexpr int kWantX = 1, kWantW = 2, kWantB = 4;
+// Up to here each small block forms the dZ it reads (a layer of 2^26 products: some 2 us of slopes, spread over the chip;
+// ReLU's cost nothing); beyond, one pass in front does.
+inline double slope_work(int act) { return act <= kRelu ? 1L << 30 : 1L << 26; }
 
 void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w, Matrix g, Matrix z,
                    int act, int want) {
     b = Backward{};
-    const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
+    b.tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
     const bool products = want & (kWantX | kWantW);
+    const bool formed = !b.tiles && (double)rows * cin * cout <= slope_work(act);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
     j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
     j.strip = strip_of(rows, cout);
     Matrix d = g;
-    const bool copy = products && (act != kNone || (tiles && !tile_operand(type, g)));
+    const bool copy = products && (b.tiles ? act != kNone || !tile_operand(type, g) : act != kNone && !formed);
     if (copy) {
-        const bool planes = tiles && type == kF32;
+        const bool planes = b.tiles && type == kF32;
         j.dst = ws.take((unsigned long)rows * j.ldd * (planes ? 6 : esize(type)));
         j.plane = planes ? rows * j.ldd : 0;
         d = Matrix{j.dst, j.ldd, rows, cout, true, j.plane};
     }
-    if (want & kWantB) {
+    b.bias_in_dw = (want & kWantB) && (want & kWantW) && !b.tiles && !copy;
+    if ((want & kWantB) && !b.bias_in_dw) {
         b.strips = (int)((rows + j.strip - 1) / j.strip);
         j.sums = b.sums = (float *)ws.take((unsigned long)b.strips * cout * 4);
     }
-    if (rows && cout && (copy || (want & kWantB))) add_job(b.jobs, b.njobs, j);
-    if (tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
-    if (tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
-    if (want & kWantX) plan(b.dx, ws, type, tiles, d, w, false, false, rows, cin, cout);
-    if (want & kWantW) plan(b.dw, ws, type, tiles, x, d, true, true, cin, cout, rows);
+    if (rows && cout && (copy || j.sums)) add_job(b.jobs, b.njobs, j);
+    if (b.tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
+    if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
+    if (want & kWantX) plan(b.dx, ws, type, b.tiles, d, w, false, false, rows, cin, cout, 64);
+    if (want & kWantW) plan(b.dw, ws, type, b.tiles, x, d, true, true, cin, cout, rows, 64);
+    if (act != kNone && !copy) {
+        for (Product *P : {&b.dx.P, &b.dw.P}) {
+            P->z = z.p; P->ldz = z.ld; P->vec_z = z.vec; P->zact = act;
+        }
+    }
+    if (b.bias_in_dw && b.dw.P.splits > 1) {
+        b.strips = b.dw.P.splits;
+        b.sums = (float *)ws.take((unsigned long)b.strips * cout * 4);
+    }
 }
 
 }  // namespace
@@ -363,7 +385,10 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     Epilogue &e = f.plan.P.e;
     e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act};
     const int rc = launch_jobs(dtype, f.jobs, f.njobs, (hipStream_t)stream);
-    return rc ? rc : launch_plan(dtype, f.plan, (hipStream_t)stream);
+    if (rc) return rc;
+    if (f.plan.edge) return launch_tile_plan(dtype, f.plan, (hipStream_t)stream);
+    const int rs = launch_small_forward(dtype, f.plan.P, (hipStream_t)stream);
+    return rs ? rs : launch_join(dtype, f.plan.P, (hipStream_t)stream);
 }
 
 extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes) {
@@ -386,7 +411,9 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     if (rows && cout && (!g || ldg < cout || (act != kNone && (!z || ldz < cout)))) return SA_ERR_INVALID;
     if ((want & kWantX) && cout && (!w || ldw < cout)) return SA_ERR_INVALID;
     if ((want & kWantW) && rows && (!x || ldx < cin)) return SA_ERR_INVALID;
-    if (((want & kWantX) && ldw >= kMaxLd) || ((want & kWantW) && ldx >= kMaxLd) || ldg >= kMaxLd) return SA_ERR_UNSUPPORTED;
+    if (((want & kWantX) && ldw >= kMaxLd) || ((want & kWantW) && ldx >= kMaxLd) || ldg >= kMaxLd ||
+        (act != kNone && ldz >= kMaxLd))
+        return SA_ERR_UNSUPPORTED;
     Backward b;
     Scratch s{(char *)ws};
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
@@ -396,23 +423,22 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_jobs(dtype, b.jobs, b.njobs, st);
     if (rc) return rc;
-    if (want & kWantB) {
-        const dim3 grid((cout + 63) / 64);
-        if (db_f32 || dtype == kF32)
-            hipLaunchKernelGGL((sum_strips_kernel<float>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (float *)db);
-        else if (dtype == kBF16)
-            hipLaunchKernelGGL((sum_strips_kernel<bf16_t>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (bf16_t *)db);
-        else
-            hipLaunchKernelGGL((sum_strips_kernel<f16_t>), grid, dim3(256), 0, st, b.sums, b.strips, cout, (f16_t *)db);
-        SA_CHECK_LAUNCH();
+    if ((want & kWantB) && !b.bias_in_dw && (rc = launch_sums(dtype, b.sums, b.strips, cout, db, db_f32, st))) return rc;
+    b.dx.P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
+    b.dw.P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
+    if (b.tiles) {
+        if ((want & kWantX) && (rc = launch_tile_plan(dtype, b.dx, st))) return rc;
+        return want & kWantW ? launch_tile_plan(dtype, b.dw, st) : SA_OK;
     }
-    if (want & kWantX) {
-        b.dx.P.e = Epilogue{dx, cin, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
-        if ((rc = launch_plan(dtype, b.dx, st))) return rc;
+    if (!(want & (kWantX | kWantW))) return SA_OK;
+    if (b.bias_in_dw) {
+        b.dw.P.colsum = db;
+        b.dw.P.col_f32 = db_f32;
+        b.dw.P.colpart = b.sums;
     }
-    if (want & kWantW) {
-        b.dw.P.e = Epilogue{dw, cout, nullptr, 0, nullptr, 0, nullptr, 0, kNone};
-        if ((rc = launch_plan(dtype, b.dw, st))) return rc;
-    }
-    return SA_OK;
+    rc = launch_small_backward(dtype, want & kWantX ? &b.dx.P : nullptr, want & kWantW ? &b.dw.P : nullptr, st);
+    if (rc) return rc;
+    if ((want & kWantX) && (rc = launch_join(dtype, b.dx.P, st))) return rc;
+    if ((want & kWantW) && (rc = launch_join(dtype, b.dw.P, st))) return rc;
+    return b.bias_in_dw && b.dw.P.splits > 1 ? launch_sums(dtype, b.sums, b.strips, cout, db, db_f32, st) : SA_OK;
 }

@@ -79,24 +79,25 @@ __device__ __forceinline__ float activate(float z, int act) {
         default: return z;
     }
 }
-// (ReLU's is a selection, made by the caller)
-__device__ __forceinline__ float act_slope(float z, int act) {
+// g act'(z).  ReLU selects: what a closed unit receives, infinities among it, does not come through.
+__device__ __forceinline__ float times_slope(float g, float z, int act) {
     switch (act) {
+        case kRelu: return z > 0.0f ? g : (z != z ? z : 0.0f);
         case kGelu: {
             float bell;
             const float tail = normal_tail(z, bell);
-            return fmaf(z * 0.39894228040143268f, bell, z >= 0.0f ? 1.0f - tail : tail);
+            return g * fmaf(z * 0.39894228040143268f, bell, z >= 0.0f ? 1.0f - tail : tail);
         }
         case kGeluTanh: {
             const float s = logistic(kGeluC * (z + kGeluA * z * z * z));
             // past |z| = 12 the logistic is 0 or 1 to every bit and the product below would be 0 times infinity
-            return fabsf(z) > 12.0f ? s : s + z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z);
+            return g * (fabsf(z) > 12.0f ? s : s + z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
         }
         case kSilu: {
             const float s = logistic(z);
-            return s + z * s * (1.0f - s);
+            return g * (s + z * s * (1.0f - s));
         }
-        default: return 1.0f;
+        default: return g;
     }
 }
 
@@ -203,6 +204,13 @@ struct Product {
     long plane_a, plane_b;   // elements between planes
     float *part;          // splits > 1: [splits][M][Np] partial sums, Np = N rounded up to a multiple of 4
     Epilogue e;
+    // small backward products
+    const void *z;        // operand G becomes G act'(z), or null
+    long ldz;
+    int vec_z, zact;
+    void *colsum;         // dW: sums of B over k, or null
+    int col_f32;
+    float *colpart;       // splits > 1: [splits][N]
 };
 __host__ __device__ inline long round_up(long v, long m) { return (v + m - 1) / m * m; }
 

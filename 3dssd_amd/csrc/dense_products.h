@@ -12,6 +12,9 @@ constexpr long kMaxTileLd = 1L << 21, kMaxLd = 1L << 24;
 // 64 k over all passes.  ta and not tb does not occur.
 int launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
 
-// Any product; P.kchunk counts k indices (a multiple of 32).
-int launch_small(int type, bool ta, bool tb, const Product &P, hipStream_t s);
+// Any forward product (A k-contiguous, B n-contiguous); P.kchunk counts k indices (a multiple of 32).
+int launch_small_forward(int type, const Product &P, hipStream_t s);
+// dX (A = G or dZ and B = W, both k-contiguous) and dW (A = X, B = G or dZ, both with rows contiguous) in one launch; either
+// may be null.  With P.z set the operand G becomes G act'(Z); dW's colsum is the bias gradient.
+int launch_small_backward(int type, const Product *dx, const Product *dw, hipStream_t s);
 }  // namespace dense

@@ -12,8 +12,11 @@
 //   t of them: which rows of the block the MFMA's 16 stand for is free, so turning the lane's 8 x N block is a few byte
 //   permutations between its own registers.
 // The n index is on the MFMA's row side: a lane holds four rows r of it at one m.
+//
+// A small layer's backward pass is one launch: dX's and dW's workgroups side by side, dZ = G act'(Z) formed in registers by
+// whoever loads G and Z, and the bias gradient summed (before dZ is rounded) by the dW workgroups of the first rows.
 #include "dense_common.h"
-#include "dense_tile.h"
+#include "dense_products.h"
 
 using namespace dense;
 
@@ -38,6 +41,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char *p) {
     return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, 0x7fffffff, 0x00020000);
 }
 
+// Elements t of a lane's words
+template <class T, class W>
+__device__ __forceinline__ float element(W v, int t) {
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (sizeof(W) == 4) return __uint_as_float(v);
+        else return __uint_as_float(v[t]);
+    } else {
+        unsigned w;
+        if constexpr (sizeof(W) <= 4) w = v;
+        else w = v[t / 2];
+        return to_f32<T>(T{(unsigned short)(t & 1 ? w >> 16 : w)});
+    }
+}
+
 // One operand of a wave's block: N blocks of 16 rows.
 template <class T, bool ROWS, int N> struct Side;
 
@@ -56,27 +73,35 @@ struct Side<T, false, N> {                             // k contiguous
             off[t] = row < rows_left ? (unsigned)((row * ld + g8) * E) : kOutside;
         }
     }
+    // left: valid k of this step, up to 32; vec: 16-byte aligned base and rows
     __device__ __forceinline__ void fetch(Regs &r, const char *base, int left, bool vec) const {
         const auto b = buffer(base);
 #pragma unroll
         for (int t = 0; t < N; ++t) {
-            if (vec && (left & 7) == 0) {              // (left: valid k of this step, up to 32)
+            if (vec && (left & 7) == 0) {
 #pragma unroll
                 for (int h = 0; h < E / 2; ++h) r.v[t][h] = load<16>(b, g8 < left ? off[t] + 16 * h : kOutside);
             } else {
 #pragma unroll
                 for (int h = 0; h < E / 2; ++h) r.v[t][h] = u4{0, 0, 0, 0};
+                if (off[t] != kOutside && g8 + 8 <= left) {
+                    __builtin_memcpy(r.v[t], base + off[t], 8 * E);    // (buffers want aligned 16 bytes, pointers do not)
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const unsigned e = load<E>(b, g8 + j < left ? off[t] + j * E : kOutside);
-                    if constexpr (E == 4) r.v[t][j / 4][j % 4] = e;
-                    else r.v[t][0][j / 2] |= j & 1 ? e << 16 : e;
+                    for (int j = 0; j < 8; ++j) {
+                        const unsigned e = load<E>(b, g8 + j < left ? off[t] + j * E : kOutside);
+                        if constexpr (E == 4) r.v[t][j / 4][j % 4] = e;
+                        else r.v[t][0][j / 2] |= j & 1 ? e << 16 : e;
+                    }
                 }
             }
         }
     }
+    static __device__ __forceinline__ float at(const Regs &r, int t, int j) {
+        if constexpr (E == 4) return __uint_as_float(r.v[t][j / 4][j % 4]);
+        else return element<T>(r.v[t][0], j);
+    }
     static __device__ __forceinline__ s8 fragment(const Regs &r, int t) { return __builtin_bit_cast(s8, r.v[t][0]); }
-    static __device__ __forceinline__ float value(const Regs &r, int t, int j) { return __uint_as_float(r.v[t][j / 4 * (E / 4)][j % 4]); }
     static __device__ __forceinline__ int row(int t, int i) { return 16 * t + i; }
 };
 
@@ -114,6 +139,7 @@ struct Side<T, true, N> {                              // rows contiguous
         if constexpr (B <= 4) return v;
         else return v[i];
     }
+    static __device__ __forceinline__ float at(const Regs &r, int t, int j) { return element<T>(r.v[j], t); }
     static __device__ __forceinline__ s8 fragment(const Regs &r, int t) {
         typename Bytes<16>::t o;
 #pragma unroll
@@ -121,69 +147,138 @@ struct Side<T, true, N> {                              // rows contiguous
             o[i] = __builtin_amdgcn_perm(word(r.v[2 * i + 1], t / 2), word(r.v[2 * i], t / 2), t & 1 ? 0x07060302 : 0x05040100);
         return __builtin_bit_cast(s8, o);
     }
-    static __device__ __forceinline__ float value(const Regs &r, int t, int j) { return __uint_as_float(word(r.v[j], t)); }
     static __device__ __forceinline__ int row(int t, int i) { return N * i + t; }
 };
 
-template <class T, bool TA, bool TB, int NA, int NB, int NW>
-__global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
-    constexpr int E = sizeof(T), kM = 16 * NA, kN = 16 * NB, kAhead = E * (NA + NB) <= 8 ? 4 : 2;
-    static_assert(NA * NB * NW <= 64, "the waves' sums: 64 KB");
-    __shared__ __attribute__((aligned(16))) float sums[NW * kM * kN];
+// What a step's products take of a side: fragments of 16-bit values, or eight fp32 values per block
+template <class T, int N> struct Operand {
+    s8 f[N];
+    __device__ __forceinline__ void set(int t, const float *v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[t][j] = (short)from_f32<T>(v[j]).u;
+    }
+};
+template <int N> struct Operand<float, N> {
+    float f[N][8];
+    __device__ __forceinline__ void set(int t, const float *v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[t][j] = v[j];
+    }
+};
+template <class T, bool ROWS, int N>
+__device__ __forceinline__ void take(Operand<T, N> &o, const typename Side<T, ROWS, N>::Regs &r) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o.f[t][j] = Side<T, ROWS, N>::at(r, t, j);
+        } else {
+            o.f[t] = Side<T, ROWS, N>::fragment(r, t);
+        }
+    }
+}
+// dZ = G act'(Z) in place of G, rounded to the type as an operand of the products; sums += the unrounded values, if wanted
+template <class T, bool ROWS, int N>
+__device__ __forceinline__ void take_slope(Operand<T, N> &o, const typename Side<T, ROWS, N>::Regs &g,
+                                           const typename Side<T, ROWS, N>::Regs &z, int act, bool summed, float *sums) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = times_slope(Side<T, ROWS, N>::at(g, t, j), Side<T, ROWS, N>::at(z, t, j), act);
+        o.set(t, d);
+        if (summed)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sums[t] += d[j];
+    }
+}
+
+template <class T, int NA, int NB>
+__device__ __forceinline__ void multiply(f4 (&acc)[NB][NA], const Operand<T, NA> &a, const Operand<T, NB> &b) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
+#pragma unroll
+                for (int x = 0; x < NA; ++x) acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(b.f[y][j], a.f[x][j], acc[y][x], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int y = 0; y < NB; ++y)
+#pragma unroll
+            for (int x = 0; x < NA; ++x) {
+                if constexpr (__is_same(T, bf16_t))
+                    acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, b.f[y]), __builtin_bit_cast(b8, a.f[x]),
+                                                                        acc[y][x], 0, 0, 0);
+                else
+                    acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b.f[y]), __builtin_bit_cast(h8, a.f[x]),
+                                                                       acc[y][x], 0, 0, 0);
+            }
+    }
+}
+
+constexpr int kSums = 64 * 256;                        // floats of LDS for the waves' sums
+
+// One workgroup's block `pos` of a product, k piece `piece`.  Z: A (ZSIDE 0) or B (ZSIDE 1) is G, and the product takes
+// G act'(Z) with Z = P.z in G's place (rows of P.ldz).
+template <class T, bool TA, bool TB, int NA, int NB, int NW, int ZSIDE>
+__device__ __forceinline__ void block_product(const Product &P, unsigned pos, int piece, float *sums) {
+    constexpr int E = sizeof(T), kM = 16 * NA, kN = 16 * NB;
+    // steps in flight, by the registers of one
+    constexpr int kSlot = 2 * E * (NA + NB + (ZSIDE == 0 ? NA : ZSIDE == 1 ? NB : 0)), kAhead = kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
+    static_assert(NW * kM * kN <= kSums, "the waves' sums");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // neighbouring blocks of n on one XCD: they share the rows of A, and with pieces below 16 bytes the lines of B
-    const unsigned q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
-    const unsigned pos = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3), nb = (unsigned)((P.N + kN - 1) / kN);
+    const unsigned nb = (unsigned)((P.N + kN - 1) / kN);
     const long m0 = (long)(pos / nb) * kM, n0 = (long)(pos % nb) * kN;
-    const long k0 = (long)blockIdx.y * P.kchunk, kend = k0 + P.kchunk < P.K ? k0 + P.kchunk : P.K;
+    const long k0 = (long)piece * P.kchunk, kend = k0 + P.kchunk < P.K ? k0 + P.kchunk : P.K;
     const char *A = (const char *)P.a + (TA ? m0 + k0 * P.lda : m0 * P.lda + k0) * E;
     const char *B = (const char *)P.b + (TB ? n0 + k0 * P.ldb : n0 * P.ldb + k0) * E;
     const long stepa = (TA ? P.lda : 1) * 32 * E, stepb = (TB ? P.ldb : 1) * 32 * E;
+    constexpr bool TZ = ZSIDE == 1 ? TB : TA;
+    constexpr int NZ = ZSIDE == 1 ? NB : NA;
+    const long z0 = ZSIDE == 1 ? n0 : m0;
+    const char *Z = (const char *)P.z + (TZ ? z0 + k0 * P.ldz : z0 * P.ldz + k0) * E;
+    const long stepz = (TZ ? P.ldz : 1) * 32 * E;
     typedef Side<T, TA, NA> SA;
     typedef Side<T, TB, NB> SB;
+    typedef Side<T, TZ, NZ> SZ;
     SA a;
     SB b;
+    SZ z;
     a.init(lane, P.lda, P.M - m0);
     b.init(lane, P.ldb, P.N - n0);
+    if (ZSIDE >= 0) z.init(lane, P.ldz, (ZSIDE == 1 ? P.N : P.M) - z0);
 
     f4 acc[NB][NA] = {};
+    float column[NB] = {};                             // sums of B's rows over k (the bias gradient), where wanted
+    const bool summed = P.colsum && m0 == 0;
     typename SA::Regs ra[kAhead];
     typename SB::Regs rb[kAhead];
+    typename SZ::Regs rz[ZSIDE >= 0 ? kAhead : 1];
     const long steps = (kend - k0 + 31) / 32;
     auto fetch = [&](int slot, long s) {
         const long l = kend - k0 - s * 32;
         const int left = l < 32 ? (int)l : 32;
         a.fetch(ra[slot], A + s * stepa, left, P.vec_a);
         b.fetch(rb[slot], B + s * stepb, left, P.vec_b);
+        if constexpr (ZSIDE >= 0) z.fetch(rz[slot], Z + s * stepz, left, P.vec_z);
     };
-    auto multiply = [&](int slot) {
-        if constexpr (E == 4) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int y = 0; y < NB; ++y)
-#pragma unroll
-                    for (int x = 0; x < NA; ++x)
-                        acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(SB::value(rb[slot], y, j), SA::value(ra[slot], x, j),
-                                                                         acc[y][x], 0, 0, 0);
+    auto products = [&](int slot) {
+        Operand<T, NA> oa;
+        Operand<T, NB> ob;
+        if constexpr (ZSIDE == 0) take_slope<T, TA, NA>(oa, ra[slot], rz[slot], P.zact, false, nullptr);
+        else take<T, TA, NA>(oa, ra[slot]);
+        if constexpr (ZSIDE == 1) {
+            take_slope<T, TB, NB>(ob, rb[slot], rz[slot], P.zact, summed, column);
         } else {
-            s8 fa[NA];
+            take<T, TB, NB>(ob, rb[slot]);
+            if (summed)
 #pragma unroll
-            for (int x = 0; x < NA; ++x) fa[x] = SA::fragment(ra[slot], x);
+                for (int t = 0; t < NB; ++t)
 #pragma unroll
-            for (int y = 0; y < NB; ++y) {
-                const s8 fb = SB::fragment(rb[slot], y);
-#pragma unroll
-                for (int x = 0; x < NA; ++x) {
-                    if constexpr (__is_same(T, bf16_t))
-                        acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, fb), __builtin_bit_cast(b8, fa[x]),
-                                                                            acc[y][x], 0, 0, 0);
-                    else
-                        acc[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, fb), __builtin_bit_cast(h8, fa[x]),
-                                                                           acc[y][x], 0, 0, 0);
-                }
-            }
+                    for (int j = 0; j < 8; ++j) column[t] += SB::at(rb[slot], t, j);
         }
+        multiply<T, NA, NB>(acc, oa, ob);
     };
     long s = wave;
 #pragma unroll
@@ -192,7 +287,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
     for (; s < steps; s += kAhead * NW) {
 #pragma unroll
         for (int h = 0; h < kAhead; ++h) {
-            if (s + h * NW < steps) multiply(h);
+            if (s + h * NW < steps) products(h);
             if (s + (h + kAhead) * NW < steps) fetch(h, s + (h + kAhead) * NW);
         }
     }
@@ -206,16 +301,17 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
                 sums[(wave * kM + SA::row(x, lane & 15)) * kN + SB::row(y, 4 * (lane >> 4) + r)] = acc[y][x][r];
     __syncthreads();
     const long Np = round_up(P.N, 4);
+    const int used = steps < NW ? (int)steps : NW;     // the others' sums are zero
 #pragma unroll 1
     for (int q = threadIdx.x; q < kM * kN / 4; q += NW * 64) {
         const int lm = q / (kN / 4), ln = q % (kN / 4) * 4;
         const long m = m0 + lm, n = n0 + ln;
         if (m >= P.M || n >= P.N) continue;
         f4 v = *(const f4 *)(sums + lm * kN + ln);
-#pragma unroll
-        for (int w = 1; w < NW; ++w) v += *(const f4 *)(sums + (w * kM + lm) * kN + ln);
+#pragma unroll 4
+        for (int w = 1; w < used; ++w) v += *(const f4 *)(sums + (w * kM + lm) * kN + ln);
         if (P.splits > 1) {
-            *(f4 *)(P.part + ((long)blockIdx.y * P.M + m) * Np + n) = v;
+            *(f4 *)(P.part + ((long)piece * P.M + m) * Np + n) = v;
         } else {
             float bias[4];
             load_bias<T, 4>(P.e, n, P.N, bias);
@@ -223,11 +319,54 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
             finish<T, 4>(P.e, m, n, P.N, o, bias);
         }
     }
+    if (summed) {                                      // four k groups of NW waves for each column
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NB; ++t) sums[(wave * 4 + (lane >> 4)) * kN + SB::row(t, lane & 15)] = column[t];
+        __syncthreads();
+        const long n = n0 + threadIdx.x;
+        if (threadIdx.x < kN && n < P.N) {
+            float v = 0.0f;
+#pragma unroll 8
+            for (int w = 0; w < 4 * NW; ++w) v += sums[w * kN + threadIdx.x];
+            if (P.splits > 1) P.colpart[(long)piece * P.N + n] = v;
+            else if (P.col_f32) ((float *)P.colsum)[n] = v;
+            else ((T *)P.colsum)[n] = from_f32<T>(v);
+        }
+    }
+}
+
+// neighbouring blocks of n on one XCD: they share the rows of A, and with pieces below 16 bytes the lines of B
+__device__ __forceinline__ unsigned on_xcd(unsigned b, unsigned blocks) {
+    const unsigned q8 = blocks >> 3, r8 = blocks & 7, xcd = b & 7;
+    return xcd * q8 + (xcd < r8 ? xcd : r8) + (b >> 3);
 }
 
 template <class T, bool TA, bool TB, int NA, int NB, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
+    __shared__ __attribute__((aligned(16))) float sums[NW * 256 * NA * NB];
+    block_product<T, TA, TB, NA, NB, NW, -1>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
+}
+
+// dX and dW of a layer in one launch: the first `nw` workgroups are dW's (all blocks of a piece, then the next piece), the
+// others dX's.  dW's blocks have WT x WT MFMA tiles.  128 registers: two workgroups of eight waves per CU.
+template <class T, bool Z, int WT, int NW>
+__global__ __launch_bounds__(NW * 64, 4) void small_backward_kernel(Product X, Product W, unsigned nw) {
+    __shared__ __attribute__((aligned(16))) float sums[NW * 1024];
+    if (blockIdx.x < nw) {
+        const unsigned blocks = nw / W.splits;
+        block_product<T, true, true, WT, WT, NW, Z ? 1 : -1>(W, on_xcd(blockIdx.x % blocks, blocks), blockIdx.x / blocks, sums);
+    } else {
+        const unsigned b = blockIdx.x - nw, blocks = (gridDim.x - nw) / X.splits;
+        block_product<T, false, false, 2, 2, NW, Z ? 0 : -1>(X, on_xcd(b % blocks, blocks), b / blocks, sums);
+    }
+}
+
+inline long blocks_of(const Product &P, long m, long n) { return ((P.M + m - 1) / m) * ((P.N + n - 1) / n); }
+
+template <class T, bool TA, bool TB, int NA, int NB, int NW>
 int launch(const Product &P, hipStream_t s) {
-    const long blocks = ((P.M + 16 * NA - 1) / (16 * NA)) * ((P.N + 16 * NB - 1) / (16 * NB));
+    const long blocks = blocks_of(P, 16 * NA, 16 * NB);
     if (blocks > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((small_kernel<T, TA, TB, NA, NB, NW>), dim3((unsigned)blocks, P.splits), dim3(NW * 64), 0, s, P);
     SA_CHECK_LAUNCH();
@@ -240,20 +379,15 @@ inline bool whole(const void *p, long ld, long rows, long c, long e) {
 }
 
 template <class T>
-int launch(bool ta, bool tb, Product P, hipStream_t s) {
+int launch_forward(Product P, hipStream_t s) {
     constexpr long E = sizeof(T);
-    if (P.M > 16 || ta || !tb) {
+    auto can = [&](long c) { return whole(P.b, P.ldb, P.N, c, E) && P.N * P.splits >= 128 * 16 * c; };
+    if (P.M > 32 || (P.M > 16 && !can(4))) {
         // blocks of 32 x 32; four waves suffice for four steps
-        const bool shorter = P.kchunk <= 128;
-        if (ta) P.vec_a = whole(P.a, P.lda, P.M, 2, E);
-        if (tb) P.vec_b = whole(P.b, P.ldb, P.N, 2, E);
-        if (ta) return shorter ? launch<T, true, true, 2, 2, 4>(P, s) : launch<T, true, true, 2, 2, 16>(P, s);
-        if (!tb) return shorter ? launch<T, false, false, 2, 2, 4>(P, s) : launch<T, false, false, 2, 2, 16>(P, s);
-        if (P.M > 32 || !whole(P.b, P.ldb, P.N, 4, E) || P.N * P.splits < 128 * 64)
-            return shorter ? launch<T, false, true, 2, 2, 4>(P, s) : launch<T, false, true, 2, 2, 16>(P, s);
+        P.vec_b = whole(P.b, P.ldb, P.N, 2, E);
+        return P.kchunk <= 128 ? launch<T, false, true, 2, 2, 4>(P, s) : launch<T, false, true, 2, 2, 16>(P, s);
     }
     // few rows: as many columns per lane as the alignment allows and as still leave 128 workgroups
-    auto can = [&](long c) { return whole(P.b, P.ldb, P.N, c, E) && P.N * P.splits >= 128 * 16 * c; };
     P.vec_b = 1;
     if (P.M > 16) {
         if constexpr (E == 2)
@@ -267,8 +401,47 @@ int launch(bool ta, bool tb, Product P, hipStream_t s) {
     return launch<T, false, true, 1, 1, 16>(P, s);
 }
 
+template <class T, bool Z, int WT, int NW>
+int launch_backward(const Product &X, const Product &W, long nx, long nw, hipStream_t s) {
+    hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW>), dim3((unsigned)(nx + nw)), dim3(NW * 64), 0, s, X, W, (unsigned)nw);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+template <class T, int WT>
+int launch_backward(const Product &X, Product W, long nx, bool z, hipStream_t s) {
+    constexpr long E = sizeof(T);
+    long nw = 0;
+    if (W.a || W.colsum || W.e.y) {
+        W.vec_a = whole(W.a, W.lda, W.M, WT, E);
+        W.vec_b = whole(W.b, W.ldb, W.N, WT, E);
+        W.vec_z = W.z && whole(W.z, W.ldz, W.N, WT, E);
+        nw = blocks_of(W, 16 * WT, 16 * WT) * W.splits;
+    }
+    if (nx + nw > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    const bool shorter = (nx == 0 || X.kchunk <= 128) && (nw == 0 || W.kchunk <= 128);
+    if (z) return shorter ? launch_backward<T, true, WT, 4>(X, W, nx, nw, s) : launch_backward<T, true, WT, 8>(X, W, nx, nw, s);
+    return shorter ? launch_backward<T, false, WT, 4>(X, W, nx, nw, s) : launch_backward<T, false, WT, 8>(X, W, nx, nw, s);
+}
+template <class T>
+int launch_backward(const Product *px, const Product *pw, hipStream_t s) {
+    Product X{}, W{};
+    X.splits = W.splits = 1;
+    if (px) X = *px;
+    if (pw) W = *pw;
+    const long nx = px ? blocks_of(X, 32, 32) * X.splits : 0;
+    const bool z = X.z || W.z;
+    // fp32 products take a CU long (16 x 16 x 4 per MFMA of 32 cycles): smaller blocks where there are few
+    if constexpr (sizeof(T) == 4)
+        if (blocks_of(W, 32, 32) * W.splits < 256) return launch_backward<T, 1>(X, W, nx, z, s);
+    return launch_backward<T, 2>(X, W, nx, z, s);
+}
+
 }  // namespace
 
-int dense::launch_small(int type, bool ta, bool tb, const Product &P, hipStream_t s) {
-    return type == kF32 ? launch<float>(ta, tb, P, s) : type == kBF16 ? launch<bf16_t>(ta, tb, P, s) : launch<f16_t>(ta, tb, P, s);
+int dense::launch_small_forward(int type, const Product &P, hipStream_t s) {
+    return type == kF32 ? launch_forward<float>(P, s) : type == kBF16 ? launch_forward<bf16_t>(P, s) : launch_forward<f16_t>(P, s);
+}
+int dense::launch_small_backward(int type, const Product *x, const Product *w, hipStream_t s) {
+    return type == kF32 ? launch_backward<float>(x, w, s) : type == kBF16 ? launch_backward<bf16_t>(x, w, s)
+                                                                         : launch_backward<f16_t>(x, w, s);
 }

@@ -16,7 +16,7 @@
 // of step t, which no wave reads any more.  One barrier per step, between the halves, orders both, and the loads have one to
 // two steps of products to arrive in.
 #include "dense_common.h"
-#include "dense_tile.h"
+#include "dense_products.h"
 
 using namespace dense;
 

@@ -81,6 +81,8 @@ def test_the_c_entries_refuse_bad_lists():
     assert lib.sa_global_norm_ws(129, ctypes.byref(n)) == 0
     two = n.value
     assert lib.sa_global_norm_ws(128, ctypes.byref(n)) == 0 and two == 2 * n.value
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses below: only where nothing could be launched on them")
     a = 1 << 20                                        # never dereferenced: every call below is refused
     ptr, num, typ = (ctypes.c_void_p * 1)(a), (ctypes.c_long * 1)(5), (ctypes.c_int * 1)(0)
     assert lib.sa_global_norm(1, ptr, num, typ, a, None, 0, None) == -1                       # no scratch
