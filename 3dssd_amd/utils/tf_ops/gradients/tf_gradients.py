@@ -8,6 +8,7 @@ the argument order and the results follow the TensorFlow functions it calls.  Th
 import bisect
 import ctypes
 import functools
+import operator
 
 import torch
 
@@ -15,6 +16,9 @@ from .. import _tensor as T
 from ... import _native as N
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_DTYPES = set(TYPES)
+_dtype_of = operator.attrgetter("dtype")
+_device_of, _address_of = torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
 def _check(t, name):
@@ -41,7 +45,9 @@ def _gather(t_list, op):
     T.require(isinstance(t_list, (list, tuple)), "%s expects a list of tensors" % op)
     ts = [t for t in t_list if t is not None]
     device = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
-    if device < 0 or not all([isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype in TYPES for t in ts]):
+    # (maps over the methods: the host's share of a call on fifty small tensors is most of its time)
+    if (device < 0 or not all([isinstance(t, torch.Tensor) for t in ts]) or not set(map(_device_of, ts)) <= {device}
+            or not set(map(_dtype_of, ts)) <= _DTYPES):
         for i, t in enumerate(t_list):                 # say which
             if t is not None:
                 _check(t, "t_list[%d]" % i)
@@ -51,8 +57,8 @@ def _gather(t_list, op):
 
 def _arrays(ts):
     k = len(ts)
-    return ((ctypes.c_void_p * k)(*[t.data_ptr() for t in ts]), (ctypes.c_long * k)(*[t.numel() for t in ts]),
-            (ctypes.c_int * k)(*[TYPES[t.dtype] for t in ts]))
+    return ((ctypes.c_void_p * k)(*map(_address_of, ts)), (ctypes.c_long * k)(*map(torch.Tensor.numel, ts)),
+            (ctypes.c_int * k)(*map(TYPES.__getitem__, map(_dtype_of, ts))))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -69,7 +75,9 @@ def _scalar_and_scratch(count, device):
 
 
 def _packed(ts):
-    return [t if t.is_contiguous() or _dense_memory(t) else t.contiguous() for t in ts]
+    if all(map(torch.Tensor.is_contiguous, ts)):
+        return ts
+    return [t if _dense_memory(t) else t.contiguous() for t in ts]
 
 
 def global_norm(t_list):
@@ -106,7 +114,7 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
         T.require(use_norm.dtype == torch.float32 and use_norm.numel() == 1, "ClipByGlobalNorm expects a float32 scalar use_norm")
     if out is None:
         ts = _packed(ts)
-        results = [torch.empty_like(t) for t in ts]
+        results = list(map(torch.empty_like, ts))
     else:
         T.require(isinstance(out, (list, tuple)) and len(out) == len(t_list), "ClipByGlobalNorm expects as many out tensors as gradients")
         in_place = out is t_list
@@ -123,7 +131,7 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
         T.require(not _overlap_between(results, moved), "ClipByGlobalNorm cannot write over another gradient")
         T.require(use_norm is None or not _overlap_between(results, [use_norm]), "ClipByGlobalNorm cannot write over use_norm")
     p, n, kinds = _arrays(ts)
-    o = (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in results])
+    o = (ctypes.c_void_p * len(ts))(*map(_address_of, results))
     if use_norm is None:
         norm, ws, size = _scalar_and_scratch(len(ts), device)
         given, to, scratch = None, norm.data_ptr(), ws.data_ptr()
