@@ -16,6 +16,8 @@
 // ran in two rounds, 115 us).
 // Longer lists: one launch of each kernel per 128 tensors, with norm_kernel between.
 // A norm that is not finite makes every output NaN, so that a step with such gradients cannot pass unseen.
+#include <stdlib.h>
+
 #include "dense_common.h"
 
 using namespace dense;
@@ -213,6 +215,42 @@ bool list_ok(int count, const void *const *p, void *const *out, bool wants_out, 
     }
     return true;
 }
+// Bytes of a tensor that is written.
+struct Span {
+    uintptr_t lo, hi;
+};
+int by_start(const void *a, const void *b) {
+    const uintptr_t x = ((const Span *)a)->lo, y = ((const Span *)b)->lo;
+    return x < y ? -1 : x > y;
+}
+bool meets(const Span *w, int count, Span r) {         // w: disjoint, in order
+    int lo = 0, hi = count;                            // the first that starts at or behind r's end
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (w[mid].lo < r.hi) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo > 0 && w[lo - 1].hi > r.lo;
+}
+// Workgroups read and write in no order: results may not overlap one another, nor anything that is read but their own
+// gradient, which they may only share whole.
+int check_overlap(int count, const void *const *p, void *const *out, const long *n, const int *type, const float *use_norm) {
+    if (count == 0) return SA_OK;
+    Span *w = (Span *)malloc(sizeof(Span) * count);
+    if (!w) return SA_ERR_INVALID;
+    int used = 0;
+    auto span = [&](const void *q, int i) { return Span{(uintptr_t)q, (uintptr_t)q + n[i] * (type[i] == kF32 ? 4 : 2)}; };
+    for (int i = 0; i < count; ++i)
+        if (n[i]) w[used++] = span(out[i], i);
+    qsort(w, used, sizeof(Span), by_start);
+    bool bad = false;
+    for (int i = 1; i < used; ++i) bad = bad || w[i].lo < w[i - 1].hi;
+    for (int i = 0; i < count && !bad; ++i)
+        if (n[i] && out[i] != p[i]) bad = meets(w, used, span(p[i], i));
+    if (!bad && use_norm) bad = meets(w, used, Span{(uintptr_t)use_norm, (uintptr_t)use_norm + 4});
+    free(w);
+    return bad ? SA_ERR_INVALID : SA_OK;
+}
 inline unsigned long ws_need(int count) { return (unsigned long)((count + kList - 1) / kList) * kBlocks * sizeof(double); }
 
 // The partial sums of the whole list; *used = how many, *lists = launches made.
@@ -257,6 +295,7 @@ extern "C" int sa_clip_by_global_norm(int count, const void *const *p, void *con
                                       float clip, const float *use_norm, float *norm, void *ws, unsigned long ws_bytes,
                                       void *stream) {
     if (!list_ok(count, p, out, true, n, type) || !(clip > 0.0f)) return SA_ERR_INVALID;
+    if (check_overlap(count, p, out, n, type, use_norm) != SA_OK) return SA_ERR_INVALID;
     hipStream_t s = (hipStream_t)stream;
     List L;
     int used = 0, lists = 0;

@@ -5,7 +5,6 @@ The reference's training graph clips every tower's gradients to a global norm of
 the argument order and the results follow the TensorFlow functions it calls.  The gradients may be of different types
 (float32, bfloat16, float16); None entries are passed over.
 """
-import bisect
 import ctypes
 import functools
 import operator
@@ -17,7 +16,7 @@ from ... import _native as N
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _DTYPES = set(TYPES)
-_dtype_of = operator.attrgetter("dtype")
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _device_of, _address_of = torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
@@ -74,10 +73,12 @@ def _scalar_and_scratch(count, device):
     return (torch.empty((), dtype=torch.float32, device=device), torch.empty(size, dtype=torch.uint8, device=device), size)
 
 
+def _all_dense(ts):
+    return all(map(torch.Tensor.is_contiguous, ts)) or all(map(_dense_memory, ts))
+
+
 def _packed(ts):
-    if all(map(torch.Tensor.is_contiguous, ts)):
-        return ts
-    return [t if _dense_memory(t) else t.contiguous() for t in ts]
+    return ts if _all_dense(ts) else [t if _dense_memory(t) else t.contiguous() for t in ts]
 
 
 def global_norm(t_list):
@@ -91,9 +92,13 @@ def global_norm(t_list):
     return norm
 
 
-def _overlap(ts):
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
-    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+def _check_results(ts, results):
+    for i, (t, o) in enumerate(zip(ts, results)):
+        _check(o, "out[%d]" % i)
+        T.require(o.shape == t.shape and o.dtype == t.dtype, "out[%d] differs from its gradient in shape or type" % i)
+        # (the stride of a dimension of one element says nothing)
+        T.require(t.numel() < 2 or all(a == b for a, b, n in zip(o.stride(), t.stride(), t.shape) if n != 1),
+                  "out[%d] differs from its gradient in strides" % i)
 
 
 def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
@@ -117,19 +122,14 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
         results = list(map(torch.empty_like, ts))
     else:
         T.require(isinstance(out, (list, tuple)) and len(out) == len(t_list), "ClipByGlobalNorm expects as many out tensors as gradients")
-        in_place = out is t_list
-        results = [o for o, t in zip(out, t_list) if t is not None]
-        for i, (t, o) in enumerate(zip(ts, results)):
-            if not in_place:
-                _check(o, "out[%d]" % i)
-                T.require(o.shape == t.shape and o.dtype == t.dtype, "out[%d] differs from its gradient in shape or type" % i)
-                T.require(t.numel() < 2 or all(a == b for a, b, n in zip(o.stride(), t.stride(), t.shape) if n != 1),
-                          "out[%d] differs from its gradient in strides" % i)
-            T.require(_dense_memory(t), "gradient %d is not dense in memory: it cannot be clipped into out" % i)
-        T.require(not _overlap(results), "ClipByGlobalNorm cannot write tensors that overlap")
-        moved = [] if in_place else [t for t, o in zip(ts, results) if t.data_ptr() != o.data_ptr()]
-        T.require(not _overlap_between(results, moved), "ClipByGlobalNorm cannot write over another gradient")
-        T.require(use_norm is None or not _overlap_between(results, [use_norm]), "ClipByGlobalNorm cannot write over use_norm")
+        if out is t_list:
+            results = ts
+        else:
+            results = [o for o, t in zip(out, t_list) if t is not None]
+            if not (all([isinstance(o, torch.Tensor) for o in results]) and set(map(_device_of, results)) <= {device} and
+                    all(list(map(f, ts)) == list(map(f, results)) for f in (_shape_of, _dtype_of, torch.Tensor.stride))):
+                _check_results(ts, results)
+        T.require(_all_dense(ts), "a gradient that is not dense in memory cannot be clipped into out")
     p, n, kinds = _arrays(ts)
     o = (ctypes.c_void_p * len(ts))(*map(_address_of, results))
     if use_norm is None:
@@ -144,17 +144,3 @@ def clip_by_global_norm(t_list, clip_norm, use_norm=None, out=None):
         return results, norm
     it = iter(results)
     return [None if t is None else next(it) for t in t_list], norm
-
-
-def _overlap_between(written, read):
-    """Does any tensor of `written` share bytes with one of `read`?  (`written` do not overlap one another.)"""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written if t.numel())
-    starts = [s[0] for s in spans]
-    for t in read:
-        if not t.numel():
-            continue
-        lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-        i = bisect.bisect_left(starts, hi) - 1       # the last written span that starts before this one ends
-        if i >= 0 and spans[i][1] > lo:
-            return True
-    return False

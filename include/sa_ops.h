@@ -274,7 +274,7 @@ int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, lo
 /* tf.global_norm / tf.clip_by_global_norm as lib/core/trainer.py:120-155 applies them: norm = sqrt(sum of squares) (64-bit
  * sums, one fp32 scalar on the device), out[i] = p[i] * clip / max(norm, clip); a norm that is not finite makes every
  * output NaN.  p, out, n (elements), type (as above): HOST arrays of `count` entries, read before the call returns.
- * out[i] == p[i] clips in place; no other overlap.  use_norm (device, nullable) replaces the list's own norm: norm and ws
+ * out[i] == p[i] clips in place; any other overlap of a result with a result, a gradient or use_norm is refused (-1).  use_norm (device, nullable) replaces the list's own norm: norm and ws
  * are then unused. */
 int sa_global_norm_ws(int count, unsigned long *bytes);
 int sa_global_norm(int count, const void *const *p, const long *n, const int *type, float *norm, void *ws,

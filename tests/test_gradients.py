@@ -96,6 +96,13 @@ def test_the_c_entries_refuse_bad_lists():
     assert lib.sa_clip_by_global_norm(1, ptr, None, num, typ, 1.0, None, a, a, n.value, None) == -1
     assert lib.sa_clip_by_global_norm(1, ptr, ptr, num, typ, 1.0, None, None, a, n.value, None) == -1
     assert lib.sa_clip_by_global_norm(1, ptr, ptr, num, typ, 1.0, None, a, a, n.value - 1, None) == -1
+    # results that overlap one another, another gradient, or the norm that is read; scratch of a later check missing
+    def pair(p0, p1, o0, o1, n0, n1, use=None):
+        return lib.sa_clip_by_global_norm(2, (ctypes.c_void_p * 2)(p0, p1), (ctypes.c_void_p * 2)(o0, o1), (ctypes.c_long * 2)(n0, n1),
+                                          (ctypes.c_int * 2)(0, 0), 1.0, use, None, None, 0, None)
+    assert pair(a, a + 400, a, a + 396, 100, 100) == -1 and pair(a, a, a, a, 100, 100) == -1
+    assert pair(a, a, a, a + 4000, 100, 100) == -1 and pair(a, a + 400, a + 400, a, 100, 100) == -1
+    assert pair(a, a + 400, a + 4, a + 8000, 100, 100) == -1 and pair(a, a + 400, a, a + 400, 100, 100, a + 796) == -1
 
 
 # --------------------------------------------------------------------------------------------------------- GPU: values
