@@ -33,7 +33,9 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
         float b[4];
         load_bias<T, 4>(P.e, n, P.N, b);
         const float v[4] = {s[0], s[1], s[2], s[3]};
-        finish<T, 4>(P.e, m, n, P.N, v, b);
+        Pack<T, 4> r{};
+        if (P.e.res) r = load_residual<T, 4>(P.e, m, n, P.N);
+        finish<T, 4>(P.e, m, n, P.N, v, b, r);
     }
 }
 
@@ -233,31 +235,50 @@ int launch_jobs(int type, Jobs &J, int n, hipStream_t s) {
     return SA_OK;
 }
 
-// A product and its k pieces.  Tiles: 256 x 256 where they fill the chip, else 128 x 128, two workgroups per CU, at least
-// four steps each.  Small: blocks of 32 x 32 up to one per CU, and pieces long enough to be worth the join's launch (4 us):
-// `least` steps of 32 k.
+// A product, its kernel and its k pieces.
 struct Plan {
     Product P;
     bool ta, tb;
-    int edge;             // of the tiles; 0: a small product
+    int shape;            // of the tiles; kNoTile: a small product
 };
-void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K,
-          long least) {
+void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K) {
     Product &P = L.P;
     L.ta = ta; L.tb = tb;
     P.M = M; P.N = N; P.K = K;
     P.a = a.p; P.lda = a.ld; P.vec_a = a.vec; P.plane_a = a.plane;
     P.b = b.p; P.ldb = b.ld; P.vec_b = b.vec; P.plane_b = b.plane;
     P.passes = type == kF32 && tiles ? 6 : 1;
-    auto count = [&](long e) { return ((M + e - 1) / e) * ((N + e - 1) / e); };
-    L.edge = !tiles ? 0 : count(256) >= 192 ? 256 : 128;
+    auto count = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
     const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
-    if (tiles) least = 4;
-    const long blocks = count(tiles ? L.edge : 32), slots = L.edge == 128 ? 512 : 256;
-    long s = slots / blocks;
-    if (s > steps / least) s = steps / least;
-    if (s < 1) s = 1;
-    long per = (steps + s - 1) / s;
+    long pieces = 1;
+    if (tiles) {
+        // The shape and the number of pieces with the least time, in units of 1 ns: rounds over the chip's slots of steps
+        // and an end each, and the join of the pieces (a launch, and the partial sums out and in at 4 TB/s).
+        static const struct { int shape, m, n, slots; double step, end; } kShapes[] = {
+            {kTile256, 256, 256, 256, 1500, 5000}, {kTile256x128, 256, 128, 256, 850, 4000}, {kTile128, 128, 128, 512, 900, 4000}};
+        double best = 0;
+        for (const auto &t : kShapes) {
+            const long c = count(t.m, t.n);
+            for (long s = 1; s == 1 || (s <= 32 && s * 4 <= steps); ++s) {
+                const long per = (steps + s - 1) / s, rounds = (c * s + t.slots - 1) / t.slots;
+                const double time = rounds * (per * t.step + t.end) + (s > 1 ? 4000 + s * (double)M * N * 8 / 4000 : 0);
+                if (best == 0 || time < best) {
+                    best = time;
+                    L.shape = t.shape;
+                    pieces = s;
+                }
+                if (c * s >= 2 * t.slots) break;
+            }
+        }
+    } else {
+        // blocks of 32 x 32 up to one per CU, in pieces long enough to be worth the join's launch
+        L.shape = kNoTile;
+        const long least = M <= 32 ? 128 : 64;
+        pieces = 256 / count(32, 32);
+        if (pieces > steps / least) pieces = steps / least;
+        if (pieces < 1) pieces = 1;
+    }
+    long per = (steps + pieces - 1) / pieces;
     if (per < 1) per = 1;
     P.splits = (int)((steps + per - 1) / per);
     if (P.splits < 1) P.splits = 1;
@@ -276,7 +297,7 @@ int launch_join(int type, const Product &P, hipStream_t s) {
     return SA_OK;
 }
 int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
-    const int rc = launch_tiles(L.edge, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
+    const int rc = launch_tiles(L.shape, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
     return rc ? rc : launch_join(type, L.P, s);
 }
 int launch_sums(int type, const float *sums, int strips, int cols, void *out, int out_f32, hipStream_t s) {
@@ -300,7 +321,7 @@ void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cou
         if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
     }
-    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin, rows <= 32 ? 128 : 64);
+    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin);
 }
 
 struct Backward {
@@ -343,8 +364,8 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     if (rows && cout && (copy || j.sums)) add_job(b.jobs, b.njobs, j);
     if (b.tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
     if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
-    if (want & kWantX) plan(b.dx, ws, type, b.tiles, d, w, false, false, rows, cin, cout, 64);
-    if (want & kWantW) plan(b.dw, ws, type, b.tiles, x, d, true, true, cin, cout, rows, 64);
+    if (want & kWantX) plan(b.dx, ws, type, b.tiles, d, w, false, false, rows, cin, cout);
+    if (want & kWantW) plan(b.dw, ws, type, b.tiles, x, d, true, true, cin, cout, rows);
     if (act != kNone && !copy) {
         for (Product *P : {&b.dx.P, &b.dw.P}) {
             P->z = z.p; P->ldz = z.ld; P->vec_z = z.vec; P->zact = act;
@@ -386,7 +407,7 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act};
     const int rc = launch_jobs(dtype, f.jobs, f.njobs, (hipStream_t)stream);
     if (rc) return rc;
-    if (f.plan.edge) return launch_tile_plan(dtype, f.plan, (hipStream_t)stream);
+    if (f.plan.shape != kNoTile) return launch_tile_plan(dtype, f.plan, (hipStream_t)stream);
     const int rs = launch_small_forward(dtype, f.plan.P, (hipStream_t)stream);
     return rs ? rs : launch_join(dtype, f.plan.P, (hipStream_t)stream);
 }

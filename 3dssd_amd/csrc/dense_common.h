@@ -66,17 +66,28 @@ __device__ __forceinline__ float normal_tail(float z, float &bell) {
     return 0.5f * bell * t * q;
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == kRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);              // NaN passes through
+    if constexpr (ACT == kGelu) {
+        float bell;
+        const float tail = normal_tail(z, bell);
+        return z * (z >= 0.0f ? 1.0f - tail : tail);
+    }
+    if constexpr (ACT == kGeluTanh) return z * logistic(kGeluC * (z + kGeluA * z * z * z));     // 0.5 (1 + tanh u) = logistic(2 u)
+    if constexpr (ACT == kSilu) return z * logistic(z);
+    return z;
+}
+// f(std::integral_constant-like tag of the activation): one branch for a whole row instead of one per element
+template <int V> struct Tag { static constexpr int value = V; };
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F &&f) {
     switch (act) {
-        case kRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);                  // NaN passes through
-        case kGelu: {
-            float bell;
-            const float tail = normal_tail(z, bell);
-            return z * (z >= 0.0f ? 1.0f - tail : tail);
-        }
-        case kGeluTanh: return z * logistic(kGeluC * (z + kGeluA * z * z * z));         // 0.5 (1 + tanh u) = logistic(2 u)
-        case kSilu: return z * logistic(z);
-        default: return z;
+        case kRelu: return f(Tag<kRelu>{});
+        case kGelu: return f(Tag<kGelu>{});
+        case kGeluTanh: return f(Tag<kGeluTanh>{});
+        case kSilu: return f(Tag<kSilu>{});
+        default: return f(Tag<kNone>{});
     }
 }
 // g act'(z).  ReLU selects: what a closed unit receives, infinities among it, does not come through.
@@ -148,48 +159,48 @@ __device__ __forceinline__ void load_bias(const Epilogue &e, long n0, long N, fl
         if (n0 + i < N) b[i] = e.bias_f32 ? ((const float *)e.bias)[n0 + i] : to_f32<T>(((const T *)e.bias)[n0 + i]);
 }
 
-// W consecutive columns n0 .. n0 + W of row m: v = the sums in fp32, b = the bias.  Each output is rounded once, from fp32.
+// W columns from n0 on of row m of the residual (zeros behind the last column), asked for ahead of finish()
 template <class T, int W>
-__device__ __forceinline__ void finish(const Epilogue &e, long m, long n0, long N, const float *v, const float *b) {
-    float z[W];
+__device__ __forceinline__ Pack<T, W> load_residual(const Epilogue &e, long m, long n0, long N) {
     Pack<T, W> p;
-    const bool whole = n0 + W <= N;
+    const T *from = (const T *)e.res + m * e.ldr + n0;
+    if (n0 + W <= N) return load_pack<T, W>(from);
 #pragma unroll
-    for (int i = 0; i < W; ++i) z[i] = v[i] + b[i];
-    if (e.pre) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) p.x[i] = from_f32<T>(z[i]);
-        T *to = (T *)e.pre + m * e.ldp + n0;
-        if (whole) store_pack<T, W>(to, p);
-        else {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (n0 + i < N) to[i] = p.x[i];
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < W; ++i) z[i] = activate(z[i], e.act);
-    if (e.res) {
-        const T *from = (const T *)e.res + m * e.ldr + n0;
-        if (whole) {
-            p = load_pack<T, W>(from);
-#pragma unroll
-            for (int i = 0; i < W; ++i) z[i] += to_f32<T>(p.x[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (n0 + i < N) z[i] += to_f32<T>(from[i]);
-        }
-    }
+    for (int i = 0; i < W; ++i) p.x[i] = n0 + i < N ? from[i] : T{};
+    return p;
+}
+
+template <class T, int W>
+__device__ __forceinline__ void store_row(T *to, const float *z, long n0, long N) {
+    Pack<T, W> p;
 #pragma unroll
     for (int i = 0; i < W; ++i) p.x[i] = from_f32<T>(z[i]);
-    T *to = (T *)e.y + m * e.ldy + n0;
-    if (whole) store_pack<T, W>(to, p);
-    else {
+    if (n0 + W <= N) {
+        store_pack<T, W>(to, p);
+    } else {
 #pragma unroll
         for (int i = 0; i < W; ++i)
             if (n0 + i < N) to[i] = p.x[i];
     }
+}
+
+// W consecutive columns n0 .. n0 + W of row m: v = the sums in fp32, b = the bias, r = the residual's columns where there is
+// one.  Each output is rounded once, from fp32.
+template <class T, int W>
+__device__ __forceinline__ void finish(const Epilogue &e, long m, long n0, long N, const float *v, const float *b, const Pack<T, W> &r) {
+    float z[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) z[i] = v[i] + b[i];
+    if (e.pre) store_row<T, W>((T *)e.pre + m * e.ldp + n0, z, n0, N);
+    with_activation(e.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] = activate<decltype(act)::value>(z[i]);
+    });
+    if (e.res) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] += to_f32<T>(r.x[i]);
+    }
+    store_row<T, W>((T *)e.y + m * e.ldy + n0, z, n0, N);
 }
 
 // ---- one product -------------------------------------------------------------------------------------------------

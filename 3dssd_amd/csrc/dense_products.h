@@ -7,10 +7,11 @@ namespace dense {
 // the 256 rows of a tile, and for the 32 of a small block (and no row is longer).
 constexpr long kMaxTileLd = 1L << 21, kMaxLd = 1L << 24;
 
-// D = A B^T on tiles of edge x edge (128 or 256) of 16-bit operands with 16-byte aligned bases and rows, and whole 16-byte
+// D = A B^T on tiles of the given shape, of 16-bit operands with 16-byte aligned bases and rows, and whole 16-byte
 // pieces along the contiguous index.  type: kBF16 / kF16 of the operands; out_type: that, or kF32.  P.kchunk counts steps of
 // 64 k over all passes.  ta and not tb does not occur.
-int launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
+enum TileShape { kNoTile = 0, kTile256 = 1, kTile256x128 = 2, kTile128 = 3 };
+int launch_tiles(int shape, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
 
 // Any forward product (A k-contiguous, B n-contiguous); P.kchunk counts k indices (a multiple of 32).
 int launch_small_forward(int type, const Product &P, hipStream_t s);

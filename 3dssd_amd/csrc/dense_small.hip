@@ -307,16 +307,20 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
         const int lm = q / (kN / 4), ln = q % (kN / 4) * 4;
         const long m = m0 + lm, n = n0 + ln;
         if (m >= P.M || n >= P.N) continue;
+        float bias[4];
+        Pack<T, 4> r{};
+        if (P.splits == 1) {
+            load_bias<T, 4>(P.e, n, P.N, bias);
+            if (P.e.res) r = load_residual<T, 4>(P.e, m, n, P.N);
+        }
         f4 v = *(const f4 *)(sums + lm * kN + ln);
 #pragma unroll 4
         for (int w = 1; w < used; ++w) v += *(const f4 *)(sums + (w * kM + lm) * kN + ln);
         if (P.splits > 1) {
             *(f4 *)(P.part + ((long)piece * P.M + m) * Np + n) = v;
         } else {
-            float bias[4];
-            load_bias<T, 4>(P.e, n, P.N, bias);
             const float o[4] = {v[0], v[1], v[2], v[3]};
-            finish<T, 4>(P.e, m, n, P.N, o, bias);
+            finish<T, 4>(P.e, m, n, P.N, o, bias, r);
         }
     }
     if (summed) {                                      // four k groups of NW waves for each column

@@ -2,8 +2,10 @@
 // that form first, dense.hip).  D(m,n) = sum_k A(m,k) B(n,k), tiles of BM x BN per workgroup, k in steps of 64.
 //
 // Both operands go from memory straight into LDS (buffer loads with an LDS destination, 16 bytes per lane, whole 128-byte
-// lines of a row).  A lane outside the operand gets an offset beyond the buffer's range, which fills its 16 bytes with zeros:
-// no edge of m, n or k needs code of its own, and nothing outside the operand is read.
+// lines of a row).  A step's buffer ends with the operand, and what lies behind its last row reads as zeros; nothing outside
+// the operand is read.  Past the last k both sides have to be zero: the buffer's end sees to it where rows run along m or n,
+// an offset beyond the buffer where they run along k.  Past the last m or n anything may be read (of the same operand): it
+// only reaches sums that are not stored.
 //   k contiguous      LDS rows of 64 k (128 bytes), whose 16-byte pieces are permuted by the row, for ds_read_b128.
 //   m / n contiguous  LDS rows of one k, whose 32-byte slots are permuted by k, for ds_read_b64_tr_b16, which transposes
 //                     4 k x 16 rows between the lanes.
@@ -15,6 +17,10 @@
 // half of step t loads A of step t + 2, into the buffer that step t - 1 has left; the second loads B of step t + 2, into that
 // of step t, which no wave reads any more.  One barrier per step, between the halves, orders both, and the loads have one to
 // two steps of products to arrive in.
+//
+// The grid is what the chip holds at once; a workgroup walks over its tiles (and pieces of k) as one sequence of steps.  The
+// loads run on into the next tile while a tile's sums leave, so only the first tile waits for memory.  The sums go through
+// LDS 16 rows at a time, in the part of the one free buffer of A that the same wave will load into next: nothing to wait for.
 #include "dense_common.h"
 #include "dense_products.h"
 
@@ -28,6 +34,8 @@ constexpr unsigned kOutside = 0x80000000u;             // past every buffer's ra
 typedef __attribute__((address_space(3))) char *lds_ptr;
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 *lds_s4;
+typedef __attribute__((address_space(3))) s8 *lds_s8;
+typedef __attribute__((address_space(3))) f4 *lds_f4;
 
 template <class MT> __device__ __forceinline__ f4 mfma(s8 a, s8 b, f4 c);
 template <> __device__ __forceinline__ f4 mfma<bf16_t>(s8 a, s8 b, f4 c) {
@@ -45,8 +53,8 @@ __device__ __forceinline__ void lds_load(u4 r, unsigned off, unsigned to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory");
 }
 
-__device__ __forceinline__ u4 buffer(const char *p) {
-    return u4{(unsigned)(uintptr_t)p, (unsigned)((uintptr_t)p >> 32) & 0xffff, 0x7fffffffu, 0x00020000u};
+__device__ __forceinline__ u4 buffer(const char *p, unsigned bytes) {
+    return u4{(unsigned)(uintptr_t)p, (unsigned)((uintptr_t)p >> 32) & 0xffff, bytes, 0x00020000u};
 }
 // s_waitcnt's code for vmcnt(n) lgkmcnt(0)
 constexpr int wait_code(int n) { return (n & 15) | (n >> 4) << 14 | 0x70; }
@@ -58,121 +66,177 @@ __device__ __forceinline__ int slot_of(int k) { return (k & 3) | ((k >> 3) & 1) 
 // Permutation of the 16-byte pieces of a row of 64 k
 __device__ __forceinline__ int piece_of(int row) { return row & 7; }
 
-// One operand's way into LDS: a tile of R rows x 64 k by W waves.
+// One operand's way into LDS: a tile of R rows x 64 k by W waves, kLoads loads of 1024 bytes each.  Load q of wave w fills
+// kilobyte q W + w: kStep rows (or k) lie between the loads of a wave, which leaves its permutation alone, so that one offset
+// per lane serves them all and the buffer moves instead.
 template <int R, int W, bool ROWS>
 struct Loader {
-    static constexpr int kLoads = R * kBK * 2 / 1024 / W;      // 1024-byte loads per wave
-    static constexpr int kPieces = R / 8;                      // 16-byte pieces of one k (ROWS)
-    unsigned off[kLoads];
-    int k[kLoads];                                             // k of the lane's piece inside a step
-    __device__ __forceinline__ void init(int wave, int lane, long ld, long rows_left) {
-#pragma unroll
-        for (int q = 0; q < kLoads; ++q) {
-            const int j = wave * kLoads + q;                   // which kilobyte of the tile
-            if (ROWS) {
-                const int b = j * 1024 + lane * 16;
-                const int kk = b / (R * 2), p = (b >> 4) & (kPieces - 1);
-                const int piece = p ^ (2 * slot_of(kk));
-                k[q] = kk;
-                off[q] = piece * 8 < rows_left ? (unsigned)(kk * ld * 2 + piece * 16) : kOutside;
-            } else {
-                const int row = j * 8 + (lane >> 3), piece = (lane & 7) ^ piece_of(row);
-                k[q] = piece * 8;
-                off[q] = row < rows_left ? (unsigned)(row * ld * 2 + piece * 16) : kOutside;
-            }
+    static constexpr int kLoads = R * kBK * 2 / 1024 / W, kStep = W * (ROWS ? 512 / R : 8);
+    static_assert(kStep % 16 == 0, "the permutations use four bits");
+    unsigned off;
+    int key;                                                   // k of the lane's piece (k contiguous)
+    __device__ __forceinline__ void init(int wave, int lane, long ld) {
+        int outer, piece;
+        if (ROWS) {
+            outer = (wave * 1024 + lane * 16) / (R * 2);
+            piece = (lane & (R / 8 - 1)) ^ (2 * slot_of(outer));
+        } else {
+            outer = wave * 8 + (lane >> 3);
+            piece = (lane & 7) ^ piece_of(outer);
         }
+        key = piece * 8;
+        off = (unsigned)(outer * ld * 2 + piece * 16);
     }
-    // Load q of this wave.  r: the tile's first row at this step's first k; k_left: valid k indices from there (none: all
-    // lanes get zeros)
-    __device__ __forceinline__ void load(u4 r, int k_left, unsigned lds, int wave, int q) const {
-        lds_load(r, k[q] < k_left ? off[q] : kOutside, lds + (wave * kLoads + q) * 1024);
+    // The bytes of a step's buffer: k and rows of it are there
+    static __device__ __forceinline__ unsigned bytes(long ld, int rows, int k) {
+        const int outer = ROWS ? k : rows, inner = ROWS ? rows : k;
+        return (unsigned)((outer - 1) * ld * 2 + ((inner * 2 + 15) & ~15));
+    }
+    // Load q; inc: the bytes of kStep rows (or k)
+    __device__ __forceinline__ void load(u4 &r, unsigned inc, int k, unsigned lds, int wave, int q) const {
+        lds_load(r, ROWS || key < k ? off : kOutside, lds + (q * W + wave) * 1024);
+        if (q + 1 < kLoads) {
+            const uint64_t p = ((uint64_t)r[1] << 32 | r[0]) + inc;
+            r[0] = (unsigned)p;
+            r[1] = (unsigned)(p >> 32);
+            const int rest = (int)r[2] - (int)inc;             // (signed, for the scalar unit: both are below 2^31)
+            r[2] = rest > 0 ? rest : 0;
+        }
     }
 };
 
-// Fragments of a wave: F blocks of 16 rows from row `first` on, 32 k each (half s of the step)
-template <int R, int F, bool ROWS>
+// Fragments of a wave: blocks of 16 rows from row `first` on (a multiple of 64), 32 k each (half s of the step).  One address
+// per wave: what a block, or a half, changes in it are bits that nothing else uses, flipped at the read.
+template <int R, bool ROWS>
 struct Reader {
-    int at[ROWS ? F : 2];
+    unsigned at;
     __device__ __forceinline__ void init(int first, int lane) {
-        const int i = lane & 15, g = lane >> 4;
-        if (ROWS) {
-            const int kk = 8 * g + (i >> 2);
-#pragma unroll
-            for (int f = 0; f < F; ++f) at[f] = kk * R * 2 + (((first / 16 + f) ^ slot_of(kk)) * 32) + (i & 3) * 8;
-        } else {
-            at[0] = (first + i) * 128 + ((g ^ piece_of(i)) * 16);
-            at[1] = at[0] ^ 64;
-        }
+        const int i = lane & 15, g = lane >> 4, kk = 8 * g + (i >> 2);
+        at = ROWS ? kk * R * 2 + (((first / 16) ^ slot_of(kk)) * 32) + (i & 3) * 8 : (first + i) * 128 + ((g ^ piece_of(i)) * 16);
     }
-    __device__ __forceinline__ s8 read(const char *lds, int f, int s) const {
+    __device__ __forceinline__ s8 read(unsigned lds, int f, int s) const {
         if (ROWS) {                                            // (k + 4 has the same permutation)
-            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at[f] + s * 64 * R));
-            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at[f] + s * 64 * R + 4 * R * 2));
+            const unsigned p = ((lds + at) ^ (f * 32)) + s * 64 * R;
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)p);
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(p + 4 * R * 2));
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
-        return *(const s8 *)(lds + at[s] + f * 2048);
+        return *(lds_s8)(uintptr_t)(((lds + at) ^ (s * 64)) + f * 2048);
     }
 };
 
 // Planes of a fp32 operand (dense.hip): which plane of A meets which of B, the smallest terms first
 __device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
 
+// f(Tag<i>): a register array's element by a number known at run time, without the array going to memory for it
+template <int I, int N, class F>
+__device__ __forceinline__ void pick(int i, F &&f) {
+    if constexpr (I + 1 < N) {
+        if (i == I) f(Tag<I>{});
+        else pick<I + 1, N>(i, f);
+    } else {
+        f(Tag<I>{});
+    }
+}
+
+// The kernel's argument, read anew: kept in scalar registers through the main loop its fields would not fit.
+__device__ __forceinline__ const Product &arguments() {
+    auto p = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Product *)(__attribute__((address_space(4))) const Product *)p;
+}
+
 template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB>
-__global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : 2) void tile_kernel(Product P) {
+__global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
     constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, kA = BM * kBK * 2, kB = BN * kBK * 2;
-    static_assert(FN % 4 == 0 && FM % 4 == 0 && W * 16384 <= 3 * kA + 2 * kB, "the epilogue takes 64 x 64 of a wave at a time");
+    static_assert(FN == 4 && kA == W * 4096, "the epilogue takes 16 x 64 of a wave at a time, in the wave's share of a buffer");
     __shared__ __attribute__((aligned(1024))) char lds[3 * kA + 2 * kB];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // tiles in groups of eight tile rows, each XCD a contiguous run of them: neighbours share operands in one L2
-    const unsigned tm = (unsigned)((P.M + BM - 1) / BM), tn = (unsigned)((P.N + BN - 1) / BN), total = tm * tn;
-    const unsigned q8 = total >> 3, r8 = total & 7, xcd = blockIdx.x & 7;
-    const unsigned pos = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
-    const unsigned group = pos / (8 * tn), in = pos - group * 8 * tn, rows = tm - group * 8 < 8 ? tm - group * 8 : 8;
-    const long m0 = (long)(group * 8 + in % rows) * BM, n0 = (long)(in / rows) * BN;
+
+    // Items: the tiles of every piece of k.  Each XCD has a contiguous run of them, its workgroups take turns; tiles go in
+    // groups of eight tile rows, so that neighbours share operands in one L2.
+    const unsigned items = (unsigned)(((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN)) * P.splits;
+    const unsigned xcd = blockIdx.x & 7, q8 = items >> 3, r8 = items & 7;
+    const unsigned stride = (gridDim.x + 7 - xcd) >> 3, end = (xcd + 1) * q8 + (xcd + 1 < r8 ? xcd + 1 : r8);
+    unsigned item = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+    struct Place {
+        long m0, n0;
+        int first, steps, piece;
+    };
+    auto place = [](const Product &P, unsigned it) {
+        const unsigned tm = (unsigned)((P.M + BM - 1) / BM), tn = (unsigned)((P.N + BN - 1) / BN), tiles = tm * tn;
+        const unsigned piece = it / tiles, pos = it - piece * tiles;
+        const unsigned group = pos / (8 * tn), in = pos - group * 8 * tn, rows = tm - group * 8 < 8 ? tm - group * 8 : 8;
+        const int all = (int)((P.K + kBK - 1) / kBK) * P.passes, first = (int)(piece * P.kchunk), left = all - first;
+        return Place{(long)(group * 8 + in % rows) * BM, (long)(in / rows) * BN, first, left < P.kchunk ? left : (int)P.kchunk, (int)piece};
+    };
 
     Loader<BM, W, TA> la;
     Loader<BN, W, TB> lb;
-    la.init(wave, lane, P.lda, P.M - m0);
-    lb.init(wave, lane, P.ldb, P.N - n0);
-    Reader<BM, FM, TA> ra;
-    Reader<BN, FN, TB> rb;
+    la.init(wave, lane, P.lda);
+    lb.init(wave, lane, P.ldb);
+    Reader<BM, TA> ra;
+    Reader<BN, TB> rb;
     const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
     ra.init(wm, lane);
     rb.init(wn, lane);
 
-    const long per = (P.K + kBK - 1) / kBK;            // steps of one pass over k
-    const long first = (long)blockIdx.y * P.kchunk, all = per * P.passes;
-    const int steps = (int)((first + P.kchunk < all ? first + P.kchunk : all) - first);
-    const char *A0 = (const char *)P.a + (TA ? m0 : m0 * P.lda) * 2, *B0 = (const char *)P.b + (TB ? n0 : n0 * P.ldb) * 2;
-    const long stepa = (TA ? P.lda : 1) * kBK * 2, stepb = (TB ? P.ldb : 1) * kBK * 2;
-
-    // the step whose loads go out: its buffers, valid k, places in LDS
-    int pass = (int)(first / per), ahead = 0;
-    long kstep = first - pass * per;
+    // The step whose loads go out: what is left of its item, its operands there, and its buffers and places in LDS.  A pass
+    // over k is `per` steps, the last of k_tail; full and tail are the bytes of the operands' buffers in either.
+    const int per = (int)((P.K + kBK - 1) / kBK), k_tail = (int)(P.K - (long)(per - 1) * kBK);
+    const int step_a = (int)(TA ? P.lda : 1) * kBK * 2, step_b = (int)(TB ? P.ldb : 1) * kBK * 2;
+    const unsigned inc_a = (unsigned)P.lda * 2 * la.kStep, inc_b = (unsigned)P.ldb * 2 * lb.kStep;
+    unsigned load_item = item;
+    int load_left = 0, pass = 0, kstep = 0, kk = 0;
+    unsigned full_a = 0, full_b = 0, tail_a = 0, tail_b = 0;
+    const char *at_a = nullptr, *at_b = nullptr;
+    u4 buf_a, buf_b;
     const unsigned base = (unsigned)(uintptr_t)(lds_ptr)lds;
     unsigned to_a = base, to_b = base + 3 * kA;
-    u4 ra_, rb_;
-    int left = 0;
+    auto start_pass = [&]() {                              // a rare one: the product's description is read again
+        const Product &R = arguments();
+        const Place p = place(R, load_item - stride);
+        at_a = (const char *)R.a + ((TA ? p.m0 : p.m0 * R.lda) + (R.passes > 1 ? kPlaneA[pass] * R.plane_a : 0)) * 2 + (long)kstep * step_a;
+        at_b = (const char *)R.b + ((TB ? p.n0 : p.n0 * R.ldb) + (R.passes > 1 ? kPlaneB[pass] * R.plane_b : 0)) * 2 + (long)kstep * step_b;
+    };
     auto next = [&]() {
-        const char *a = A0 + kstep * stepa, *b = B0 + kstep * stepb;
-        if (P.passes > 1 && pass < 6) {
-            a += kPlaneA[pass] * P.plane_a * 2;
-            b += kPlaneB[pass] * P.plane_b * 2;
+        if (load_left == 0 && load_item < end) {
+            const Product &R = arguments();
+            const Place p = place(R, load_item);
+            load_item += stride;
+            load_left = p.steps;
+            pass = p.first / per;
+            kstep = p.first - pass * per;
+            const int rows_a = R.M - p.m0 < BM ? (int)(R.M - p.m0) : BM, rows_b = R.N - p.n0 < BN ? (int)(R.N - p.n0) : BN;
+            full_a = la.bytes(R.lda, rows_a, kBK);
+            full_b = lb.bytes(R.ldb, rows_b, kBK);
+            tail_a = la.bytes(R.lda, rows_a, k_tail);
+            tail_b = lb.bytes(R.ldb, rows_b, k_tail);
+            start_pass();
         }
-        ra_ = buffer(a);
-        rb_ = buffer(b);
-        const long k_left = P.K - kstep * kBK;
-        left = ahead >= steps ? 0 : k_left < kBK ? (int)k_left : kBK;
-        ++ahead;
-        if (++kstep == per) kstep = 0, ++pass;
+        const bool some = load_left != 0, last = kstep == per - 1;     // past the last item: zeros, from nowhere
+        kk = last ? k_tail : kBK;
+        buf_a = buffer(at_a, some ? last ? tail_a : full_a : 0);
+        buf_b = buffer(at_b, some ? last ? tail_b : full_b : 0);
+        if (some) {
+            --load_left;
+            ++kstep;
+            at_a += step_a;
+            at_b += step_b;
+            if (last && load_left) {
+                kstep = 0;
+                ++pass;
+                start_pass();
+            }
+        }
     };
     constexpr int LA = Loader<BM, W, TA>::kLoads, LB = Loader<BN, W, TB>::kLoads;
     auto load_a = [&](int q) {
-        la.load(ra_, left, to_a, wave, q);
+        la.load(buf_a, inc_a, kk, to_a, wave, q);
         if (q == LA - 1) to_a = to_a == base + 2 * kA ? base : to_a + kA;
     };
     auto load_b = [&](int q) {
-        lb.load(rb_, left, to_b, wave, q);
+        lb.load(buf_b, inc_b, kk, to_b, wave, q);
         if (q == LB - 1) to_b = base + 3 * kA + kB - (to_b - base - 3 * kA);
     };
 
@@ -181,13 +245,13 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : 2) void tile
     constexpr int kOps = FM + FN + (LA > LB ? LA : LB), kEvery = FM * FN / kOps;
     static_assert(kEvery >= 1, "an operation per product at most");
     struct Fragments { s8 a[FM], b[FN]; };
-    f4 acc[FN][FM] = {};
+    f4 acc[FN][FM];
     Fragments f0, f1;
-    auto read = [&](Fragments &f, const char *a, const char *b, int s, int op) {
+    auto read = [&](Fragments &f, unsigned a, unsigned b, int s, int op) {
         if (op < FN) f.b[op] = rb.read(b, op, s);
         else f.a[op - FN] = ra.read(a, op - FN, s);
     };
-    auto half = [&](Fragments &use, Fragments &get, const char *a, const char *b, int s, auto &&load, int loads) {
+    auto half = [&](Fragments &use, Fragments &get, unsigned a, unsigned b, int s, auto &&load, int loads) {
 #pragma unroll
         for (int x = 0; x < FM * FN; ++x) {
             const int j = x / FM, i = x % FM;
@@ -211,67 +275,145 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 256 ? WM * WN / 4 : 2) void tile
     // loads return in order: with those of step 1 outstanding, step 0's have arrived
     __builtin_amdgcn_s_waitcnt(wait_code(LA + LB));
     __builtin_amdgcn_s_barrier();
-    const char *a0 = lds, *b0 = lds + 3 * kA;          // this step's buffers
+    unsigned a0 = base, b0 = base + 3 * kA;            // this step's buffers
+    for (; item < end; item += stride) {
+        const int steps = place(arguments(), item).steps;
+        // (the last half before read these too; kept from there they would take 48 registers through the end of the tile)
 #pragma unroll
-    for (int op = 0; op < FM + FN; ++op) read(f0, a0, b0, 0, op);
-    for (int step = 0; step < steps; ++step) {
-        next();
-        half(f0, f1, a0, b0, 1, load_a, LA);
-        // step + 1 has arrived (this wave's part; the barrier makes it everyone's), and everyone has read all of this step
-        __builtin_amdgcn_s_waitcnt(wait_code(LA));
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        a0 = a0 == lds + 2 * kA ? lds : a0 + kA;
-        b0 = lds + 3 * kA + kB - (b0 - lds - 3 * kA);
-        half(f1, f0, a0, b0, 0, load_b, LB);
-    }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                // the zeros of the steps past the end have arrived too
+        for (int op = 0; op < FM + FN; ++op) read(f0, a0, b0, 0, op);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[j][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int step = 0; step < steps; ++step) {
+            next();
+            half(f0, f1, a0, b0, 1, load_a, LA);
+            // step + 1 has arrived (this wave's part; the barrier makes it everyone's), and everyone has read all of this one
+            __builtin_amdgcn_s_waitcnt(wait_code(LA));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            a0 = a0 == base + 2 * kA ? base : a0 + kA;
+            b0 = base + 3 * kA + kB - (b0 - base - 3 * kA);
+            half(f1, f0, a0, b0, 0, load_b, LB);
+        }
 
-    // The sums leave through LDS, 64 x 64 of a wave at a time (16 KB of its own): the epilogue's code then exists once, and
-    // eight lanes write 128 neighbouring bytes (16-bit) of a row.  16-byte pieces of a row are permuted by ^ row & 15.
-    const long Np = round_up(P.N, 4);
-    char *mine = lds + wave * 16384;
-    __syncthreads();
+        // The sums: 16 rows of the wave's 64 columns at a time, through 4 KB of LDS (16-byte pieces of a row permuted by ^ row),
+        // so that eight lanes write 128 neighbouring bytes (16-bit) of a row.
+        const Product &R = arguments();
+        int l = lane;                                  // (computed from anew: kept, its offsets would take main loop registers)
+        asm volatile("" : "+v"(l));
+        const Place p = place(R, item);
+        const long n = p.n0 + wn + (l & 7) * 8, mw = p.m0 + wm + (l >> 3), N = R.N, M = R.M;
+        const unsigned mine = to_a + wave * 1024;      // kilobytes wave, W + wave, ..: four rows each
+        const unsigned put = mine + ((l & 15) >> 2) * (W * 1024) + (l & 3) * 256, take = mine + (l >> 5) * (W * 1024) + ((l >> 3) & 3) * 256;
+        auto leave = [&](int i) __attribute__((always_inline)) {       // blocks i of the wave's columns into LDS
+            pick<0, FM>(i, [&](auto block) __attribute__((always_inline)) {
+                constexpr int b = decltype(block)::value;
+                const unsigned g = l >> 4, x = l & 15;
+                f4 v[4] = {acc[0][b], acc[1][b], acc[2][b], acc[3][b]};
+                // (branches that only differ in where they read the array from would be made one, and the array memory)
+                asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *(lds_f4)(uintptr_t)(put + (((4 * j + g) ^ x) * 16)) = v[j];
+            });
+        };
+        auto row = [&](int q, float *v) __attribute__((always_inline)) {              // columns n .. n + 8 of row 8 q + l / 8 of them
+            const int r = 8 * q + (l >> 3), piece = (l & 7) * 2;
+            const f4 lo = *(lds_f4)(uintptr_t)(take + q * 2 * (W * 1024) + ((piece ^ r) * 16));
+            const f4 hi = *(lds_f4)(uintptr_t)(take + q * 2 * (W * 1024) + (((piece + 1) ^ r) * 16));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = lo[c], v[4 + c] = hi[c];
+        };
+        if (R.splits > 1) {
+            const long Np = round_up(N, 4);
+            float *to = R.part + ((long)p.piece * M + mw) * Np + n;
 #pragma unroll 1
-    for (int h = 0; h < FM * FN / 16; ++h) {
+            for (int i = 0; i < FM; ++i) {
+                leave(i);
 #pragma unroll
-        for (int hh = 0; hh < FM * FN / 16; ++hh)
-            if (hh == h) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int row = 16 * i + (lane & 15), piece = (4 * j + (lane >> 4)) ^ (lane & 15);
-                        *(f4 *)(mine + row * 256 + piece * 16) = acc[4 * (hh / (FM / 4)) + j][4 * (hh % (FM / 4)) + i];
+                for (int q = 0; q < 2; ++q, to += 8 * Np) {
+                    float v[8];
+                    row(q, v);
+                    if (mw + 16 * i + 8 * q < M) {
+                        if (n < N) *(f4 *)to = f4{v[0], v[1], v[2], v[3]};
+                        if (n + 4 < N) *(f4 *)(to + 4) = f4{v[4], v[5], v[6], v[7]};
                     }
+                }
             }
-        const long n = n0 + wn + 64 * (h / (FM / 4)) + (lane & 7) * 8, mh = m0 + wm + 64 * (h % (FM / 4));
-        float bias[8];
-        load_bias<OT, 8>(P.e, n, P.N, bias);           // (none in a product whose sums are joined later)
+        } else if (p.n0 + BN <= N) {
+            // whole columns: no lane looks at the edge, and the activation is chosen once
+            const Epilogue &E = R.e;
+            const long ldy = E.ldy, ldp = E.ldp, ldr = E.ldr;
+            OT *to = (OT *)E.y + mw * ldy + n, *pre = (OT *)E.pre + mw * ldp + n;
+            const OT *res = (const OT *)E.res + mw * ldr + n;
+            const bool has_pre = E.pre, has_res = E.res;
+            float bias[8];
+            load_bias<OT, 8>(E, n, N, bias);
+            Pack<OT, 8> r[2] = {};
+            auto ask = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q, res += 8 * ldr)
+                    if (mw + 16 * i + 8 * q < M) r[q] = load_pack<OT, 8>(res);
+            };
+            if (has_res) ask(0);
+            with_activation(E.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll 1
-        for (int q = 0; q < 8; ++q) {
-            const int row = q * 8 + (lane >> 3), piece = (lane & 7) * 2;
-            const f4 lo = *(const f4 *)(mine + row * 256 + ((piece ^ (row & 15)) * 16));
-            const f4 hi = *(const f4 *)(mine + row * 256 + (((piece + 1) ^ (row & 15)) * 16));
-            const long m = mh + row;
-            if (m >= P.M || n >= P.N) continue;
-            if (P.splits > 1) {
-                float *p = P.part + ((long)blockIdx.y * P.M + m) * Np + n;
-                *(f4 *)p = lo;
-                if (n + 4 < P.N) *(f4 *)(p + 4) = hi;
-            } else {
-                const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                finish<OT, 8>(P.e, m, n, P.N, v, bias);
+                for (int i = 0; i < FM; ++i) {
+                    leave(i);
+                    const Pack<OT, 8> now[2] = {r[0], r[1]};
+                    if (has_res && i + 1 < FM) ask(i + 1);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q, to += 8 * ldy, pre += 8 * ldp) {
+                        float z[8];
+                        row(q, z);
+                        if (mw + 16 * i + 8 * q >= M) continue;
+                        Pack<OT, 8> o;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) z[c] += bias[c];
+                        if (has_pre) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) o.x[c] = from_f32<OT>(z[c]);
+                            store_pack<OT, 8>(pre, o);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) z[c] = activate<decltype(act)::value>(z[c]);
+                        if (has_res) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) z[c] += to_f32<OT>(now[q].x[c]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) o.x[c] = from_f32<OT>(z[c]);
+                        store_pack<OT, 8>(to, o);
+                    }
+                }
+            });
+        } else {
+            float bias[8];
+            load_bias<OT, 8>(R.e, n, N, bias);
+#pragma unroll 1
+            for (int i = 0; i < FM; ++i) {
+                leave(i);
+#pragma unroll 1
+                for (int q = 0; q < 2; ++q) {
+                    const long m = mw + 16 * i + 8 * q;
+                    float v[8];
+                    row(q, v);
+                    if (m >= M || n >= N) continue;
+                    Pack<OT, 8> r{};
+                    if (R.e.res) r = load_residual<OT, 8>(R.e, m, n, N);
+                    finish<OT, 8>(R.e, m, n, N, v, bias, r);
+                }
             }
         }
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                // the zeros of the steps past the end have arrived too
 }
 
 template <int BM, int BN, int WM, int WN, class MT, class OT>
-int launch(bool ta, bool tb, const Product &P, hipStream_t s) {
-    const long tiles = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN);
-    if (tiles > 0x3fffffffL) return SA_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)tiles, P.splits), block(WM * WN * 64);
+int launch(bool ta, bool tb, const Product &P, int slots, hipStream_t s) {
+    const long items = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN) * P.splits;
+    if (items > 0x3fffffffL) return SA_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(items < slots ? items : slots)), block(WM * WN * 64);
     if (ta) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, true, true>), grid, block, 0, s, P);
     else if (tb) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, true>), grid, block, 0, s, P);
     else hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, false>), grid, block, 0, s, P);
@@ -280,15 +422,16 @@ int launch(bool ta, bool tb, const Product &P, hipStream_t s) {
 }
 
 template <class MT, class OT>
-int launch(int edge, bool ta, bool tb, const Product &P, hipStream_t s) {
-    if (edge == 256) return launch<256, 256, 2, 4, MT, OT>(ta, tb, P, s);
-    return launch<128, 128, 2, 2, MT, OT>(ta, tb, P, s);
+int launch(int shape, bool ta, bool tb, const Product &P, hipStream_t s) {
+    if (shape == kTile256) return launch<256, 256, 2, 4, MT, OT>(ta, tb, P, 256, s);
+    if (shape == kTile256x128) return launch<256, 128, 4, 2, MT, OT>(ta, tb, P, 256, s);
+    return launch<128, 128, 2, 2, MT, OT>(ta, tb, P, 512, s);
 }
 
 }  // namespace
 
-int dense::launch_tiles(int edge, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s) {
-    if (out_type == kF32) return launch<bf16_t, float>(edge, ta, tb, P, s);
-    if (type == kBF16) return launch<bf16_t, bf16_t>(edge, ta, tb, P, s);
-    return launch<f16_t, f16_t>(edge, ta, tb, P, s);
+int dense::launch_tiles(int shape, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s) {
+    if (out_type == kF32) return launch<bf16_t, float>(shape, ta, tb, P, s);
+    if (type == kBF16) return launch<bf16_t, bf16_t>(shape, ta, tb, P, s);
+    return launch<f16_t, f16_t>(shape, ta, tb, P, s);
 }
