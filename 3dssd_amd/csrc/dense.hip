@@ -11,9 +11,9 @@ namespace {
 template <class T> using Eight = Pack<T, 8>;
 
 // Columns c .. c + 8 of a row; zeros behind the last column.
-template <class T>
+template <class T, bool WHOLE>
 __device__ __forceinline__ Eight<T> fetch(const T *row, int c, int cols) {
-    if (c + 8 <= cols) return load_pack<T, 8>(row + c);
+    if constexpr (WHOLE) return load_pack<T, 8>(row + c);
     Eight<T> v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.x[i] = c + i < cols ? row[c + i] : T{};
@@ -49,8 +49,9 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
 //   or, of a fp32 matrix, three bf16 planes x = h + m + l, each the rounded rest of the one before: 27 bits, so nothing of
 //   x's 24 is lost, and the six products h h, h m, m h, m m, h l, l h of two such operands leave out terms below 2^-24 of
 //   the product -- fp32's own rounding -- at 6 / 16 of the cost of fp32 MFMAs.
-// A thread owns eight columns of every eighth row of its block's strip; the eight row lanes of a block meet in LDS, the
-// strips in sum_strips_kernel, in a fixed order.  Bound by memory: each element is read and written once.
+// A thread owns eight columns; a block's threads take 256 columns of eight rows at a time, or of wide matrices 2048 of one
+// (4 KB runs of 16-bit elements).  The row lanes of a block meet in LDS, the strips in
+// sum_strips_kernel, in a fixed order.  Bound by memory: each element is read and written once.
 struct Job {
     const void *g, *z;    // z null: no activation
     long ldg, ldz;
@@ -62,6 +63,7 @@ struct Job {
     long plane;           // elements between planes; 0: one copy in the layer's type
     float *sums;          // [strips][cols], or null
     long strip;           // rows of a block
+    int wide;             // 2048 columns of a row at a time
 };
 struct Jobs {
     Job j[3];
@@ -87,55 +89,72 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
     const int which = blockIdx.x >= J.first[2] ? 2 : blockIdx.x >= J.first[1] ? 1 : 0;
     const Job S = J.j[which];
     const long blk = blockIdx.x - J.first[which];
-    const int cb = (S.cols + 255) / 256, bx = (int)(blk % cb);
+    const int span = S.wide ? 2048 : 256, lanes = S.wide ? 1 : 8;      // columns and rows that a block takes at a time
+    const int cb = (S.cols + span - 1) / span, bx = (int)(blk % cb);
     const long by = blk / cb;
-    const int c0 = bx * 256 + (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    const int c0 = bx * span + (S.wide ? threadIdx.x : threadIdx.x & 31) * 8, rl = S.wide ? 0 : threadIdx.x >> 5;
     const long r0 = by * S.strip, r1 = r0 + S.strip < S.rows ? r0 + S.strip : S.rows;
     float sum[8] = {};
     constexpr int kRows = 4;                           // rows in flight per thread
-    for (long r = r0 + rl; r < r1 && c0 < S.cols; r += 8 * kRows) {
-        Eight<T> g[kRows], z[kRows];
+    // whole: all of the thread's columns are there.  (A branch per load instead lets the compiler share its first elements with
+    // the partial case and cut the 16-byte load to pieces.)
+    auto walk = [&](auto act, auto whole) __attribute__((always_inline)) {
+        constexpr int A = decltype(act)::value;
+        constexpr bool kWhole = decltype(whole)::value;
+        for (long r = r0 + rl; r < r1 && c0 < S.cols; r += lanes * kRows) {
+            Eight<T> g[kRows], z[kRows];
 #pragma unroll
-        for (int u = 0; u < kRows; ++u)
-            if (r + 8 * u < r1) {
-                g[u] = fetch((const T *)S.g + (r + 8 * u) * S.ldg, c0, S.cols);
-                if (S.z) z[u] = fetch((const T *)S.z + (r + 8 * u) * S.ldz, c0, S.cols);
-            }
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            if (r + 8 * u >= r1) break;
-            float d[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = to_f32<T>(g[u].x[i]);
-            if (S.z) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = times_slope(d[i], to_f32<T>(z[u].x[i]), S.act);
-            }
-            if (S.dst) {
-                const long at = (r + 8 * u) * S.ldd + c0;
-                if (sizeof(T) == 4 && S.plane) {
-                    Eight<bf16_t> o[3];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        unsigned short h[3];
-                        three_planes(d[i], h);
-#pragma unroll
-                        for (int p = 0; p < 3; ++p) o[p].x[i].u = h[p];
-                    }
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) store_pack<bf16_t, 8>((bf16_t *)S.dst + p * S.plane + at, o[p]);
-                } else {
-                    Eight<T> o;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
-                    store_pack<T, 8>((T *)S.dst + at, o);
+            for (int u = 0; u < kRows; ++u)
+                if (r + lanes * u < r1) {
+                    g[u] = fetch<T, kWhole>((const T *)S.g + (r + lanes * u) * S.ldg, c0, S.cols);
+                    if (A != kNone) z[u] = fetch<T, kWhole>((const T *)S.z + (r + lanes * u) * S.ldz, c0, S.cols);
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += d[i];
+            for (int u = 0; u < kRows; ++u) {
+                if (r + lanes * u >= r1) break;
+                float d[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = to_f32<T>(g[u].x[i]);
+                if (A != kNone) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[i] = times_slope<A>(d[i], to_f32<T>(z[u].x[i]));
+                }
+                if (S.dst) {
+                    const long at = (r + lanes * u) * S.ldd + c0;
+                    if (sizeof(T) == 4 && S.plane) {
+                        Eight<bf16_t> o[3];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            unsigned short h[3];
+                            three_planes(d[i], h);
+#pragma unroll
+                            for (int p = 0; p < 3; ++p) o[p].x[i].u = h[p];
+                        }
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) store_pack<bf16_t, 8>((bf16_t *)S.dst + p * S.plane + at, o[p]);
+                    } else {
+                        Eight<T> o;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o.x[i] = from_f32<T>(d[i]);
+                        store_pack<T, 8>((T *)S.dst + at, o);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += d[i];
+            }
         }
-    }
+    };
+    with_activation(S.z ? S.act : kNone, [&](auto act) __attribute__((always_inline)) {
+        if (c0 + 8 <= S.cols) walk(act, Tag<1>{});
+        else walk(act, Tag<0>{});
+    });
     if (!S.sums) return;
+    if (S.wide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < S.cols) S.sums[by * S.cols + c0 + i] = sum[i];
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[rl][(threadIdx.x & 31) * 8 + i] = sum[i];
     __syncthreads();
@@ -192,26 +211,32 @@ struct Matrix {
 // The tile kernel's loads are 16 bytes of 16-bit elements
 inline bool tile_operand(int type, const Matrix &m) { return type != kF32 && m.vec && m.cols % 8 == 0; }
 
-// Does a layer of this size go to the tile kernel?  The small kernel's time against the tiles' (us): fp32 512^3 8 / 24,
-// 1024^3 41 / 39, 2048 x 1024 x 1024 77 / 55; bf16 512^3 7 / 12, 1024 x 512 x 512 12 / 13, 1024^3 25 / 22; where the operands
-// have to be copied first 511^3 11 / 15, 1023^3 70 / 27.  A tile of 128 rows is no place for 32.
-inline bool wants_tiles(int type, long rows, int cin, int cout, bool copies) {
-    const double least = type == kF32 ? 1L << 30 : copies ? 1L << 28 : 1L << 29;
-    return rows > 32 && cin > 32 && cout > 32 && (double)rows * cin * cout >= least && cin < kMaxTileLd && cout < kMaxTileLd;
+// Does a layer of this size go to the tile kernel?  The small kernel's time against the tiles' (us): fp32 1024 x 512 x 512
+// 14 / 26, 1024^3 42 / 36; bf16 1024 x 512 x 512 11 / 11, 1024 x 1024 x 512 12 / 14, 1024^3 22 / 15; where the operands have to
+// be copied first 701^3 18 / 19, 1023^3 54 / 25; gradients 1024^3 fp32 64 / 69, bf16 35 / 37, 701^3 32 / 36.  Few rows are no
+// work for a tile of 128, least of all where a fp32 W has to be split first (64 x 4096 x 4096 30 / 74).
+inline bool wants_tiles(int type, long rows, int cin, int cout, bool copies, bool backward) {
+    // (backward: two products, for which the small kernel needs one launch and no copies)
+    const double least = backward ? (copies && type != kF32 ? 7e8 : 1.3e9) : type == kF32 ? 9e8 : copies ? 4e8 : 6e8;
+    return rows > (type == kF32 ? 128 : 32) && cin > 32 && cout > 32 && (double)rows * cin * cout >= least && cin < kMaxTileLd &&
+           cout < kMaxTileLd;
 }
-
 // Makes the copy (or planes) of m that the products read, as one of J's jobs
 void add_job(Jobs &J, int &n, Job j) {
     J.j[n] = j;
-    J.first[n + 1] = J.first[n] + (long)((j.cols + 255) / 256) * ((j.rows + j.strip - 1) / j.strip);
+    const int span = j.wide ? 2048 : 256;
+    J.first[n + 1] = J.first[n] + (long)((j.cols + span - 1) / span) * ((j.rows + j.strip - 1) / j.strip);
     ++n;
 }
-// Rows of a block: a thousand blocks where the matrix has them, and no more strips than 512
-long strip_of(long rows, int cols) {
-    long s = rows * ((cols + 255) / 256) / 1024;
-    if (s > 63) s = 63;
-    if (s < rows / 512) s = rows / 512;
-    return round_up(s + 1, 8);
+// Whether a block takes 2048 columns at a time, and its rows: a thousand blocks or more where the matrix has them, and no more
+// strips than 512.
+void shape_job(Job &j) {
+    j.wide = j.cols >= 2048 && (j.cols % 2048 == 0 || j.cols >= 8192);
+    const int span = j.wide ? 2048 : 256, lanes = j.wide ? 1 : 8;
+    long s = j.rows * ((j.cols + span - 1) / span) / 1024;
+    if (!j.wide && s > 63) s = 63;
+    if (s < j.rows / 512) s = j.rows / 512;
+    j.strip = round_up(s + 1, lanes);
 }
 void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
     Job j{};
@@ -219,7 +244,7 @@ void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
     j.ldd = round_up(m.cols, 8);
     j.plane = type == kF32 ? m.rows * j.ldd : 0;
     j.dst = ws.take((unsigned long)m.rows * j.ldd * 2 * (type == kF32 ? 3 : 1));
-    j.strip = strip_of(m.rows, m.cols);
+    shape_job(j);
     m = Matrix{j.dst, j.ldd, m.rows, m.cols, true, j.plane};
     add_job(J, n, j);
 }
@@ -252,22 +277,25 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
     long pieces = 1;
     if (tiles) {
-        // The shape and the number of pieces with the least time, in units of 1 ns: rounds over the chip's slots of steps
-        // and an end each, and the join of the pieces (a launch, and the partial sums out and in at 4 TB/s).
-        static const struct { int shape, m, n, slots; double step, end; } kShapes[] = {
-            {kTile256, 256, 256, 256, 1500, 5000}, {kTile256x128, 256, 128, 256, 850, 4000}, {kTile128, 128, 128, 512, 900, 4000}};
+        // The shape and the number of pieces with the least time (ns): rounds over the chip's slots, each of the piece's steps
+        // and a tile's end -- a step takes longer the more of the chip works (alone / full: measured on bf16, products of
+        // 1024^3 to 8192^3) -- and the join of the pieces: a launch, and the partial sums out and in at 8 TB/s.
+        static const struct { int shape, m, n, slots; double alone, full, end; } kShapes[] = {
+            {kTile256, 256, 256, 256, 1050, 1430, 8500}, {kTile256x128, 256, 128, 256, 690, 840, 5500}, {kTile128, 128, 128, 512, 400, 890, 5000}};
         double best = 0;
         for (const auto &t : kShapes) {
             const long c = count(t.m, t.n);
             for (long s = 1; s == 1 || (s <= 32 && s * 4 <= steps); ++s) {
-                const long per = (steps + s - 1) / s, rounds = (c * s + t.slots - 1) / t.slots;
-                const double time = rounds * (per * t.step + t.end) + (s > 1 ? 4000 + s * (double)M * N * 8 / 4000 : 0);
+                const long per = (steps + s - 1) / s, items = c * s, rounds = items / t.slots, rest = items % t.slots;
+                double time = rounds * (per * t.full + t.end);
+                if (rest) time += per * (t.alone + (t.full - t.alone) * rest / t.slots) + t.end;
+                if (s > 1) time += 4000 + s * (double)M * N / 1000;
                 if (best == 0 || time < best) {
                     best = time;
                     L.shape = t.shape;
                     pieces = s;
                 }
-                if (c * s >= 2 * t.slots) break;
+                if (items >= 2 * t.slots) break;
             }
         }
     } else {
@@ -316,7 +344,7 @@ struct Forward {
 };
 void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w) {
     f = Forward{};
-    const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
+    const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w), false);
     if (tiles) {
         if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
@@ -341,13 +369,13 @@ inline double slope_work(int act) { return act <= kRelu ? 1L << 30 : 1L << 26; }
 void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w, Matrix g, Matrix z,
                    int act, int want) {
     b = Backward{};
-    b.tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w));
+    b.tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w), true);
     const bool products = want & (kWantX | kWantW);
     const bool formed = !b.tiles && (double)rows * cin * cout <= slope_work(act);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
     j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
-    j.strip = strip_of(rows, cout);
+    shape_job(j);
     Matrix d = g;
     const bool copy = products && (b.tiles ? act != kNone || !tile_operand(type, g) : act != kNone && !formed);
     if (copy) {

@@ -91,25 +91,24 @@ __device__ __forceinline__ void with_activation(int act, F &&f) {
     }
 }
 // g act'(z).  ReLU selects: what a closed unit receives, infinities among it, does not come through.
-__device__ __forceinline__ float times_slope(float g, float z, int act) {
-    switch (act) {
-        case kRelu: return z > 0.0f ? g : (z != z ? z : 0.0f);
-        case kGelu: {
-            float bell;
-            const float tail = normal_tail(z, bell);
-            return g * fmaf(z * 0.39894228040143268f, bell, z >= 0.0f ? 1.0f - tail : tail);
-        }
-        case kGeluTanh: {
-            const float s = logistic(kGeluC * (z + kGeluA * z * z * z));
-            // past |z| = 12 the logistic is 0 or 1 to every bit and the product below would be 0 times infinity
-            return g * (fabsf(z) > 12.0f ? s : s + z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
-        }
-        case kSilu: {
-            const float s = logistic(z);
-            return g * (s + z * s * (1.0f - s));
-        }
-        default: return g;
+template <int ACT>
+__device__ __forceinline__ float times_slope(float g, float z) {
+    if constexpr (ACT == kRelu) return z > 0.0f ? g : (z != z ? z : 0.0f);
+    if constexpr (ACT == kGelu) {
+        float bell;
+        const float tail = normal_tail(z, bell);
+        return g * fmaf(z * 0.39894228040143268f, bell, z >= 0.0f ? 1.0f - tail : tail);
     }
+    if constexpr (ACT == kGeluTanh) {
+        const float s = logistic(kGeluC * (z + kGeluA * z * z * z));
+        // past |z| = 12 the logistic is 0 or 1 to every bit and the product below would be 0 times infinity
+        return g * (fabsf(z) > 12.0f ? s : s + z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
+    }
+    if constexpr (ACT == kSilu) {
+        const float s = logistic(z);
+        return g * (s + z * s * (1.0f - s));
+    }
+    return g;
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------

@@ -184,8 +184,11 @@ __device__ __forceinline__ void take_slope(Operand<T, N> &o, const typename Side
 #pragma unroll
     for (int t = 0; t < N; ++t) {
         float d[8];
+        with_activation(act, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = times_slope(Side<T, ROWS, N>::at(g, t, j), Side<T, ROWS, N>::at(z, t, j), act);
+            for (int j = 0; j < 8; ++j)
+                d[j] = times_slope<decltype(a)::value>(Side<T, ROWS, N>::at(g, t, j), Side<T, ROWS, N>::at(z, t, j));
+        });
         o.set(t, d);
         if (summed)
 #pragma unroll
