@@ -70,16 +70,23 @@ struct Jobs {
     long first[4];        // blocks of the jobs
 };
 
-// x finite and too large for bf16 rounds to its largest value (the planes below hold the rest); an infinity has no rest
+// x finite and too large for bf16 rounds to its largest value (the planes below hold the rest).  An infinity is
+// (+-1, 0, +-infinity): the last plane only meets the other factor's first, which has its sign and is 0 only if the factor
+// is; in the first plane it would meet rests that are 0 or of the other sign, and the sum would be NaN.
 __device__ __forceinline__ void three_planes(float x, unsigned short (&o)[3]) {
     float r = x;
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         unsigned short h = from_f32<bf16_t>(r).u;
-        if ((h & 0x7fff) == 0x7f80 && fabsf(r) <= 3.402823466e38f) h -= 1;
+        if ((h & 0x7fff) == 0x7f80) h -= 1;
         o[i] = h;
-        const float f = __uint_as_float((unsigned)h << 16);
-        r = fabsf(f) <= 3.402823466e38f ? r - f : (f != f ? f : 0.0f);
+        r -= __uint_as_float((unsigned)h << 16);
+    }
+    if (fabsf(x) == __builtin_inff()) {
+        const unsigned short sign = x < 0.0f ? 0x8000 : 0;
+        o[0] = sign | 0x3f80;
+        o[1] = 0;
+        o[2] = sign | 0x7f80;
     }
 }
 

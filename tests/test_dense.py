@@ -325,6 +325,35 @@ def test_infinities_and_nans_stay_in_their_rows_and_columns(gpu, dt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", [(3, 512, 256), (257, 131, 67), (1024, 1024, 1024), (1031, 1021, 1027)])
+def test_infinities_have_the_sign_of_the_product(gpu, dt, size):
+    """One infinite factor among finite ones gives an infinity of the product's sign, two of opposite signs and infinity times
+    zero NaN -- also where the other factor has few bits (1) or many, is large or small.  (The exact sums are rounded to the
+    type first: fp16 has no 86462.)"""
+    m = _mod()
+    rows, cin, cout = size
+    inf = float("inf")
+    x, w = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2)
+    w[3, :40:2], w[3, 1:41:2] = 1.0, -1.0                  # what the infinities below meet
+    w[3, 41:50] = torch.tensor([0.0, 3e4, -3e4, 1.001, -1.001, 3e-5, -3e-5, 511.5, -511.5], device=gpu).to(dt)
+    x[:, 5] = torch.where(x[:, 5] == 0, torch.ones((), dtype=dt, device=gpu), x[:, 5])
+    x[2, 5] = 0.0
+    x[1, 3], x[rows - 1, 3] = inf, -inf
+    w[5, 7], w[5, 60] = -inf, inf
+    x[rows // 2, 5] = inf                                  # meets the infinities of w
+    out, expected = m.dense(x, w), (x.double() @ w.double()).to(dt)
+    for ours, theirs in ((torch.isnan(out), torch.isnan(expected)), (out == inf, expected == inf), (out == -inf, expected == -inf)):
+        assert torch.equal(ours, theirs)
+    g = _rand(gpu, (rows, cout), dt, 3)
+    g[1, 3], g[rows - 1, 5] = inf, -inf
+    dx, dw, _ = m.dense_grad(x, w, g)
+    for out, expected in ((dx, (g.double() @ w.double().T).to(dt)), (dw, (x.double().T @ g.double()).to(dt))):
+        for ours, theirs in ((torch.isnan(out), torch.isnan(expected)), (out == inf, expected == inf), (out == -inf, expected == -inf)):
+            assert torch.equal(ours, theirs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("size", [(5, 64, 40), (131, 67, 259), (300, 512, 264), (2048, 512, 128)])
 def test_nothing_is_written_outside_the_outputs(gpu, dt, size):
     lib, m = pkg("utils._native").lib(), _mod()
