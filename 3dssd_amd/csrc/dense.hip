@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void sum_strips_kernel(const float *sums, int 
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 inline long esize(int type) { return type == kF32 ? 4 : 2; }
-inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld < kMaxTileLd; }
+inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld * esize(type) < 2 * kMaxTileLd; }
 inline bool sizes_ok(int type, long rows, int cin, int cout) {
     return type >= kF32 && type <= kF16 && rows >= 0 && cin >= 0 && cout >= 0 && cin < kMaxLd && cout < kMaxLd;
 }
@@ -211,7 +211,7 @@ struct Matrix {
     const void *p;
     long ld, rows;
     int cols;
-    bool vec;             // 16-byte aligned base and rows, fewer than kMaxTileLd elements apart
+    bool vec;             // 16-byte aligned base and rows, less than 4 MB apart
     long plane = 0;
 };
 
@@ -245,12 +245,12 @@ void shape_job(Job &j) {
     if (s < j.rows / 512) s = j.rows / 512;
     j.strip = round_up(s + 1, lanes);
 }
-void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m) {
+void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m, bool planes = true) {
     Job j{};
     j.g = m.p; j.ldg = m.ld; j.rows = m.rows; j.cols = m.cols;
     j.ldd = round_up(m.cols, 8);
-    j.plane = type == kF32 ? m.rows * j.ldd : 0;
-    j.dst = ws.take((unsigned long)m.rows * j.ldd * 2 * (type == kF32 ? 3 : 1));
+    j.plane = type == kF32 && planes ? m.rows * j.ldd : 0;
+    j.dst = ws.take((unsigned long)m.rows * j.ldd * (j.plane ? 6 : esize(type)));
     shape_job(j);
     m = Matrix{j.dst, j.ldd, m.rows, m.cols, true, j.plane};
     add_job(J, n, j);
@@ -273,24 +273,26 @@ struct Plan {
     bool ta, tb;
     int shape;            // of the tiles; kNoTile: a small product
 };
-void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Matrix &b, bool ta, bool tb, long M, long N, long K) {
+enum Kind { kSmall, kTiles, kSplit };
+// Chooses shape and pieces; returns the time to expect (ns; tiles only).
+double plan(Plan &L, int type, Kind kind, bool ta, bool tb, long M, long N, long K) {
     Product &P = L.P;
     L.ta = ta; L.tb = tb;
     P.M = M; P.N = N; P.K = K;
-    P.a = a.p; P.lda = a.ld; P.vec_a = a.vec; P.plane_a = a.plane;
-    P.b = b.p; P.ldb = b.ld; P.vec_b = b.vec; P.plane_b = b.plane;
-    P.passes = type == kF32 && tiles ? 6 : 1;
+    P.passes = type == kF32 && kind == kTiles ? 6 : 1;
     auto count = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
-    const long unit = tiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
+    const long unit = kind == kTiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
     long pieces = 1;
-    if (tiles) {
+    double best = 0;
+    if (kind != kSmall) {
         // The shape and the number of pieces with the least time (ns): rounds over the chip's slots, each of the piece's steps
         // and a tile's end -- a step takes longer the more of the chip works (alone / full: measured on bf16, products of
         // 1024^3 to 8192^3) -- and the join of the pieces: a launch, and the partial sums out and in at 8 TB/s.
         static const struct { int shape, m, n, slots; double alone, full, end; } kShapes[] = {
-            {kTile256, 256, 256, 256, 1050, 1430, 8500}, {kTile256x128, 256, 128, 256, 690, 840, 5500}, {kTile128, 128, 128, 512, 400, 890, 5000}};
-        double best = 0;
+            {kTile256, 256, 256, 256, 1050, 1430, 8500}, {kTile256x128, 256, 128, 256, 690, 840, 5500},
+            {kTile128, 128, 128, 512, 400, 890, 5000}, {kSplit256, 256, 256, 256, 2700, 3300, 8500}};
         for (const auto &t : kShapes) {
+            if ((t.shape == kSplit256) != (kind == kSplit)) continue;
             const long c = count(t.m, t.n);
             for (long s = 1; s == 1 || (s <= 32 && s * 4 <= steps); ++s) {
                 const long per = (steps + s - 1) / s, items = c * s, rounds = items / t.slots, rest = items % t.slots;
@@ -317,8 +319,15 @@ void plan(Plan &L, Scratch &ws, int type, bool tiles, const Matrix &a, const Mat
     if (per < 1) per = 1;
     P.splits = (int)((steps + per - 1) / per);
     if (P.splits < 1) P.splits = 1;
-    P.kchunk = tiles ? per : per * 32;
-    P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * M * round_up(N, 4) * 4) : nullptr;
+    P.kchunk = kind == kSmall ? per * 32 : per;
+    return best;
+}
+// The operands, and room for the pieces' sums
+void place(Plan &L, Scratch &ws, const Matrix &a, const Matrix &b) {
+    Product &P = L.P;
+    P.a = a.p; P.lda = a.ld; P.vec_a = a.vec; P.plane_a = a.plane;
+    P.b = b.p; P.ldb = b.ld; P.vec_b = b.vec; P.plane_b = b.plane;
+    P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * P.M * round_up(P.N, 4) * 4) : nullptr;
 }
 
 int launch_join(int type, const Product &P, hipStream_t s) {
@@ -332,7 +341,8 @@ int launch_join(int type, const Product &P, hipStream_t s) {
     return SA_OK;
 }
 int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
-    const int rc = launch_tiles(L.shape, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
+    const int rc = L.shape == kSplit256 ? launch_split(L.tb, L.P, s)
+                                        : launch_tiles(L.shape, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
     return rc ? rc : launch_join(type, L.P, s);
 }
 int launch_sums(int type, const float *sums, int strips, int cols, void *out, int out_f32, hipStream_t s) {
@@ -352,11 +362,22 @@ struct Forward {
 void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w) {
     f = Forward{};
     const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w), false);
+    const double time = plan(f.plan, type, tiles ? kTiles : kSmall, false, true, rows, cout, cin);
+    if (tiles && type == kF32) {
+        // x as it is, or copied once for its alignment, where that beats its planes (10 bytes an element, at 4.5 TB/s)
+        const bool direct = x.vec && cin % 4 == 0;
+        Plan split{};
+        const double other = plan(split, type, kSplit, false, true, rows, cout, cin);
+        if ((direct || round_up(cin, 8) < kMaxTileLd / 2) && other < time + (double)rows * cin * (direct ? 10 : 2) / 4500) {
+            f.plan = split;
+            if (!direct) copy_for_tiles(f.jobs, f.njobs, ws, type, x, false);
+        }
+    }
     if (tiles) {
-        if (!tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
+        if (f.plan.shape != kSplit256 && !tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
     }
-    plan(f.plan, ws, type, tiles, x, w, false, true, rows, cout, cin);
+    place(f.plan, ws, x, w);
 }
 
 struct Backward {
@@ -399,8 +420,15 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     if (rows && cout && (copy || j.sums)) add_job(b.jobs, b.njobs, j);
     if (b.tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
     if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
-    if (want & kWantX) plan(b.dx, ws, type, b.tiles, d, w, false, false, rows, cin, cout);
-    if (want & kWantW) plan(b.dw, ws, type, b.tiles, x, d, true, true, cin, cout, rows);
+    const Kind kind = b.tiles ? kTiles : kSmall;
+    if (want & kWantX) {
+        plan(b.dx, type, kind, false, false, rows, cin, cout);
+        place(b.dx, ws, d, w);
+    }
+    if (want & kWantW) {
+        plan(b.dw, type, kind, true, true, cin, cout, rows);
+        place(b.dw, ws, x, d);
+    }
     if (act != kNone && !copy) {
         for (Product *P : {&b.dx.P, &b.dw.P}) {
             P->z = z.p; P->ldz = z.ld; P->vec_z = z.vec; P->zact = act;

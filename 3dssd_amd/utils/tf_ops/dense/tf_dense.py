@@ -95,7 +95,7 @@ def _stream(device):
 
 
 def _aligned(ptr, ld, itemsize):
-    return ptr % 16 == 0 and ld * itemsize % 16 == 0 and ld < 1 << 21
+    return ptr % 16 == 0 and ld * itemsize % 16 == 0 and ld * itemsize < 1 << 22
 
 
 def dense(inputs, weights, biases=None, activation=None, residual=None, return_preact=False):

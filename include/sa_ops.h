@@ -258,7 +258,7 @@ int sa_dense(long rows, int K, int N, const float *x, const void *wpack, const f
  * 4 SiLU.  Any alignments of whole elements; cin, cout and the
  * strides below 2^24 (-3 otherwise); sums in fp32, one rounding per output, no atomics: the
  * same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has a 16-byte aligned base
- * and rows fewer than 2^21 elements apart), 256-byte aligned, used until the call's work on the stream is done. */
+ * and rows less than 4 MB apart), 256-byte aligned, used until the call's work on the stream is done. */
 int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes);
 int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
                      const void *bias, int bias_f32, const void *res, long ldr, int act, void *y, void *pre, void *ws,

@@ -187,6 +187,26 @@ def test_dense_matches_64_bits(gpu, size, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pad", [0, 1, 4])
+@pytest.mark.parametrize("size", [(600, 1020, 1604), (1031, 1021, 1027), (32773, 44, 700), (7000, 68, 2100), (150, 6004, 1029),
+                                  (66000, 96, 256)])
+def test_large_fp32_products_at_odd_places(gpu, size, pad):
+    """Lengths that end inside a step of 32, rows 16-byte aligned and not, kept sums, a residual, and none."""
+    m = _mod()
+    rows, cin, cout = size
+    i = rows + pad
+    big = _rand(gpu, (rows, cin + pad), torch.float32, i)
+    big[:, :pad] = float("nan")
+    x, w = big[:, pad:], _rand(gpu, (cin, cout), torch.float32, i + 1, math.sqrt(2.0 / cin))
+    b, res = _rand(gpu, (cout,), torch.float32, i + 2), _rand(gpu, (rows, cout), torch.float32, i + 3)
+    out, pre = m.dense(x, w, b, activation="silu", residual=res, return_preact=True)
+    _check_forward(x, w, b, "silu", res, out, pre)
+    plain = m.dense(x, w)
+    _check_forward(x, w, None, None, None, plain, None)
+    assert torch.equal(m.dense(x, w), plain)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 def test_every_activation_over_its_whole_range(gpu, act, dt):
