@@ -1,6 +1,6 @@
 // The dense layer on plain weights: y = act(x W + b) + residual in fp32, bf16 or fp16, and its gradient
 // (dense_common.h has the formulas).  This file: the pass in front of the products that need one, the join of split sums,
-// the choice of kernel, and the C ABI.  The products are in dense_products.hip (large) and dense_small.hip.
+// the choice of kernel, and the C ABI.  The products are in dense_tile.hip and dense_split.hip (large) and dense_small.hip.
 #include "dense_common.h"
 #include "dense_products.h"
 
@@ -286,11 +286,11 @@ double plan(Plan &L, int type, Kind kind, bool ta, bool tb, long M, long N, long
     double best = 0;
     if (kind != kSmall) {
         // The shape and the number of pieces with the least time (ns): rounds over the chip's slots, each of the piece's steps
-        // and a tile's end -- a step takes longer the more of the chip works (alone / full: measured on bf16, products of
-        // 1024^3 to 8192^3) -- and the join of the pieces: a launch, and the partial sums out and in at 8 TB/s.
+        // and a tile's end -- a step takes longer the more of the chip works (alone / full: measured on bf16, kSplit256 on fp32,
+        // products of 1024^3 to 8192^3) -- and the join of the pieces: a launch, and the partial sums out and in at 8 TB/s.
         static const struct { int shape, m, n, slots; double alone, full, end; } kShapes[] = {
             {kTile256, 256, 256, 256, 1050, 1430, 8500}, {kTile256x128, 256, 128, 256, 690, 840, 5500},
-            {kTile128, 128, 128, 512, 400, 890, 5000}, {kSplit256, 256, 256, 256, 2700, 3300, 8500}};
+            {kTile128, 128, 128, 512, 400, 890, 5000}, {kSplit256, 256, 256, 256, 2700, 4150, 8500}};
         for (const auto &t : kShapes) {
             if ((t.shape == kSplit256) != (kind == kSplit)) continue;
             const long c = count(t.m, t.n);
@@ -341,7 +341,7 @@ int launch_join(int type, const Product &P, hipStream_t s) {
     return SA_OK;
 }
 int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
-    const int rc = L.shape == kSplit256 ? launch_split(L.tb, L.P, s)
+    const int rc = L.shape == kSplit256 ? launch_split(L.P, s)
                                         : launch_tiles(L.shape, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
     return rc ? rc : launch_join(type, L.P, s);
 }

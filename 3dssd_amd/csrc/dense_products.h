@@ -1,4 +1,4 @@
-// Interface between dense.hip and the kernels for large (dense_tile.hip) and small products (dense_small.hip).
+// Interface between dense.hip and the kernels for large (dense_tile.hip, dense_split.hip) and small products (dense_small.hip).
 #pragma once
 #include "dense_common.h"
 
@@ -14,9 +14,9 @@ enum TileShape { kNoTile = 0, kTile256 = 1, kTile256x128 = 2, kTile128 = 3, kSpl
 int launch_tiles(int shape, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
 
 // A in fp32 (k contiguous, 16-byte aligned base and rows, fewer than kMaxTileLd / 2 elements apart, K a multiple of 4 or
-// zeros behind it up to one), B as three bf16 planes like the tiles' operands, to fp32, on tiles of 256 x 256; P.passes is 1
+// zeros behind it up to one), B as three bf16 planes (n contiguous, like the tiles' operands), to fp32, on tiles of 256 x 256; P.passes is 1
 // and P.kchunk counts steps of 32 k.
-int launch_split(bool tb, const Product &P, hipStream_t s);
+int launch_split(const Product &P, hipStream_t s);
 
 // Any forward product (A k-contiguous, B n-contiguous); P.kchunk counts k indices (a multiple of 32).
 int launch_small_forward(int type, const Product &P, hipStream_t s);

@@ -189,7 +189,7 @@ def test_dense_matches_64_bits(gpu, size, dt):
 @pytest.mark.gpu
 @pytest.mark.parametrize("pad", [0, 1, 4])
 @pytest.mark.parametrize("size", [(600, 1020, 1604), (1031, 1021, 1027), (32773, 44, 700), (7000, 68, 2100), (150, 6004, 1029),
-                                  (66000, 96, 256)])
+                                  (66000, 96, 256), (8192, 2052, 68), (16400, 1028, 72), (9000, 2600, 300)])
 def test_large_fp32_products_at_odd_places(gpu, size, pad):
     """Lengths that end inside a step of 32, rows 16-byte aligned and not, kept sums, a residual, and none."""
     m = _mod()
@@ -345,7 +345,7 @@ def test_infinities_and_nans_stay_in_their_rows_and_columns(gpu, dt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("size", [(3, 512, 256), (257, 131, 67), (1024, 1024, 1024), (1031, 1021, 1027)])
+@pytest.mark.parametrize("size", [(3, 512, 256), (257, 131, 67), (1024, 1024, 1024), (1031, 1021, 1027), (33000, 128, 256)])
 def test_infinities_have_the_sign_of_the_product(gpu, dt, size):
     """One infinite factor among finite ones gives an infinity of the product's sign, two of opposite signs and infinity times
     zero NaN -- also where the other factor has few bits (1) or many, is large or small.  (The exact sums are rounded to the
