@@ -59,7 +59,7 @@ struct Job {
     long rows;
     int cols;
     void *dst;            // [rows][ldd], or null: sums only
-    long ldd;             // cols rounded up to a multiple of 8
+    long ldd;             // copied_ld(cols)
     long plane;           // elements between planes; 0: one copy in the layer's type
     float *sums;          // [strips][cols], or null
     long strip;           // rows of a block
@@ -228,6 +228,10 @@ inline bool wants_tiles(int type, long rows, int cin, int cout, bool copies, boo
     return rows > (type == kF32 ? 128 : 32) && cin > 32 && cout > 32 && (double)rows * cin * cout >= least && cin < kMaxTileLd &&
            cout < kMaxTileLd;
 }
+// Rows of a copy begin on a line of the caches, so that a step's 128 bytes of one are not on two: the tile kernel takes
+// 30.4 us instead of 32.9 for 5003 x 771 x 1283.  (Behind the zeros up to a multiple of 8 nothing is written, and nothing is read that matters.)
+inline long copied_ld(long cols) { return round_up(cols, 64); }
+
 // Makes the copy (or planes) of m that the products read, as one of J's jobs
 void add_job(Jobs &J, int &n, Job j) {
     J.j[n] = j;
@@ -248,7 +252,7 @@ void shape_job(Job &j) {
 void copy_for_tiles(Jobs &J, int &n, Scratch &ws, int type, Matrix &m, bool planes = true) {
     Job j{};
     j.g = m.p; j.ldg = m.ld; j.rows = m.rows; j.cols = m.cols;
-    j.ldd = round_up(m.cols, 8);
+    j.ldd = copied_ld(m.cols);
     j.plane = type == kF32 && planes ? m.rows * j.ldd : 0;
     j.dst = ws.take((unsigned long)m.rows * j.ldd * (j.plane ? 6 : esize(type)));
     shape_job(j);
@@ -368,7 +372,7 @@ void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cou
         const bool direct = x.vec && cin % 4 == 0;
         Plan split{};
         const double other = plan(split, type, kSplit, false, true, rows, cout, cin);
-        if ((direct || round_up(cin, 8) < kMaxTileLd / 2) && other < time + (double)rows * cin * (direct ? 10 : 2) / 4500) {
+        if ((direct || copied_ld(cin) < kMaxTileLd / 2) && other < time + (double)rows * cin * (direct ? 10 : 2) / 4500) {
             f.plan = split;
             if (!direct) copy_for_tiles(f.jobs, f.njobs, ws, type, x, false);
         }
@@ -402,7 +406,7 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     const bool formed = !b.tiles && (double)rows * cin * cout <= slope_work(act);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
-    j.rows = rows; j.cols = cout; j.ldd = round_up(cout, 8);
+    j.rows = rows; j.cols = cout; j.ldd = copied_ld(cout);
     shape_job(j);
     Matrix d = g;
     const bool copy = products && (b.tiles ? act != kNone || !tile_operand(type, g) : act != kNone && !formed);
