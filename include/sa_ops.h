@@ -255,10 +255,10 @@ int sa_dense(long rows, int K, int N, const float *x, const void *wpack, const f
 /* y = act(x W + bias) + res.  dtype: 0 fp32, 1 bf16, 2 fp16, of x [rows,cin] (ldx elements between rows), W [cin,cout]
  * (ldw), res [rows,cout] (ldr; nullable), y and pre [rows,cout] (dense; pre = x W + bias, nullable); bias [cout] (nullable)
  * is fp32 where bias_f32 is set, else of that type.  act: 0 none, 1 ReLU, 2 GELU (normal integral), 3 GELU (tanh form),
- * 4 SiLU.  Any alignments of whole elements; cin, cout and the
- * strides below 2^24 (-3 otherwise); sums in fp32, one rounding per output, no atomics: the
- * same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has a 16-byte aligned base
- * and rows less than 4 MB apart), 256-byte aligned, used until the call's work on the stream is done. */
+ * 4 SiLU.  Any alignments of whole elements; cin, cout and the strides below 2^24 (-3 otherwise); sums in fp32, one
+ * rounding per output, no atomics: the same call gives the same bits.  ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 =
+ * x / W has a 16-byte aligned base and row length, and rows less than 4 MB apart), 256-byte aligned, used until the call's
+ * work on the stream is done. */
 int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes);
 int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
                      const void *bias, int bias_f32, const void *res, long ldr, int act, void *y, void *pre, void *ws,
@@ -274,8 +274,8 @@ int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, lo
 /* tf.global_norm / tf.clip_by_global_norm as lib/core/trainer.py:120-155 applies them: norm = sqrt(sum of squares) (64-bit
  * sums, one fp32 scalar on the device), out[i] = p[i] * clip / max(norm, clip); a norm that is not finite makes every
  * output NaN.  p, out, n (elements), type (as above): HOST arrays of `count` entries, read before the call returns.
- * out[i] == p[i] clips in place; any other overlap of a result with a result, a gradient or use_norm is refused (-1).  use_norm (device, nullable) replaces the list's own norm: norm and ws
- * are then unused. */
+ * out[i] == p[i] clips in place; any other overlap of a result with a result, a gradient or use_norm is refused (-1).
+ * use_norm (device, nullable) replaces the list's own norm: norm and ws are then unused. */
 int sa_global_norm_ws(int count, unsigned long *bytes);
 int sa_global_norm(int count, const void *const *p, const long *n, const int *type, float *norm, void *ws,
                    unsigned long ws_bytes, sa_stream_t stream);

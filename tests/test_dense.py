@@ -374,7 +374,7 @@ def test_infinities_have_the_sign_of_the_product(gpu, dt, size):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("size", [(5, 64, 40), (131, 67, 259), (300, 512, 264), (2048, 512, 128)])
+@pytest.mark.parametrize("size", [(5, 64, 40), (131, 67, 259), (300, 512, 264), (2048, 512, 128), (33003, 132, 259)])
 def test_nothing_is_written_outside_the_outputs(gpu, dt, size):
     lib, m = pkg("utils._native").lib(), _mod()
     rows, cin, cout = size
@@ -428,12 +428,29 @@ def test_offsets_past_32_bits(gpu):
     _check_grad(x[-100:], w, out[-100:], None, None, None, dw, None)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,cin,cout", [(torch.float32, 1100, 40), (torch.bfloat16, 2200, 40), (torch.bfloat16, 40, 2200)])
+def test_large_products_with_offsets_past_32_bits(gpu, dt, cin, cout):
+    m = _mod()
+    rows = (1 << 20) + 70                              # inputs, or results, of more than 2^32 bytes
+    x, g = torch.zeros(rows, cin, dtype=dt, device=gpu), torch.zeros(rows, cout, dtype=dt, device=gpu)
+    w = _rand(gpu, (cin, cout), dt, 1, 0.05)
+    x[-100:], g[-100:] = _rand(gpu, (100, cin), dt, 2), _rand(gpu, (100, cout), dt, 3)
+    out = m.dense(x, w)
+    _check_forward(x[-100:], w, None, None, None, out[-100:], None)
+    assert not bool(out[:-100].any())
+    del out
+    dx, dw, _ = m.dense_grad(x, w, g)
+    assert not bool(dx[:-100].any())
+    _check_grad(x[-100:], w, g[-100:], None, None, dx[-100:], dw, None)
+
+
 # ------------------------------------------------------------------------------------------- GPU: streams, graphs, refusals
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
 def test_other_streams_and_captured_graphs_give_the_same_bits(gpu, dt):
     m = _mod()
-    for rows, cin, cout in ((1, 1024, 512), (515, 771, 259), (512, 512, 512)):
+    for rows, cin, cout in ((1, 1024, 512), (515, 771, 259), (512, 512, 512), (33003, 129, 257)):
         x, w, b = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2, 0.05), _rand(gpu, (cout,), dt, 3)
         g = _rand(gpu, (rows, cout), dt, 4)
 

@@ -231,3 +231,15 @@ def test_refused_lists(gpu):
             m.clip_by_global_norm(ts, 1.0, **kw)
     got, norm = m.clip_by_global_norm([a, a], 1.0)      # the same gradient twice counts twice
     _check([a, a], 1.0, got, norm)
+
+
+@pytest.mark.gpu
+def test_a_tensor_of_more_than_32_bits_of_elements(gpu):
+    m = _mod()
+    t = torch.zeros((1 << 31) + 77, dtype=torch.bfloat16, device=gpu)
+    t[:2], t[-3:] = 3.0, 4.0
+    assert abs(float(m.global_norm([t])) - 66.0 ** 0.5) <= 2.0 ** -23 * 66.0 ** 0.5
+    m.clip_by_global_norm([t], 1.0, out=[t])
+    # one division of 64 bits, two roundings to fp32 and one to bf16
+    assert all(abs(float(v) - want / 66.0 ** 0.5) <= 2.0 ** -7.9 * want / 66.0 ** 0.5 for v, want in ((t[0], 3.0), (t[-1], 4.0)))
+    assert int((t != 0).sum()) == 5
