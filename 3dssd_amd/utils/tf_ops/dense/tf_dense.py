@@ -70,7 +70,7 @@ def _layer(op, inputs, weights, biases, activation):
     """Checks what both functions take; (type, cin, cout, device).  One pass over the conditions in the ordinary case: the
     messages are only made where one of them does not hold."""
     if not (isinstance(inputs, torch.Tensor) and isinstance(weights, torch.Tensor) and inputs.is_cuda and
-            inputs.get_device() == weights.get_device() == torch.cuda.current_device() and
+            inputs.get_device() == weights.get_device() == torch._C._cuda_getDevice() and
             inputs.dtype == weights.dtype and inputs.dtype in TYPES):
         _operand(inputs, "inputs")
         _operand(weights, "weights", inputs.dtype)
@@ -79,13 +79,13 @@ def _layer(op, inputs, weights, biases, activation):
     if weights.dim() != 2:
         raise ValueError("%s expects (cin,cout) weights shape" % op)
     cin, cout = weights.shape
-    if inputs.dim() == 0 or inputs.shape[-1] != cin:
+    if inputs.dim() == 0 or inputs.size(-1) != cin:
         raise ValueError("%s expects (...,cin) inputs shape" % op)
-    if max(cin, cout) >= _FAR:
+    if cin >= _FAR or cout >= _FAR:
         raise ValueError("%s expects fewer than 2**24 channels" % op)
     if biases is not None:
         _beside(biases, "biases", inputs, torch.float32)
-        if biases.shape != (cout,):
+        if biases.dim() != 1 or biases.size(0) != cout:
             raise ValueError("%s expects (cout) biases shape" % op)
     return inputs.dtype, cin, cout
 
@@ -107,7 +107,7 @@ def dense(inputs, weights, biases=None, activation=None, residual=None, return_p
     dense_grad needs.  Rows may lie apart (any stride, last dimension contiguous); other layouts are copied first.
     An input of no rows gives an empty result; with cin = 0 the product is zero."""
     dt, cin, cout = _layer("Dense", inputs, weights, biases, activation)
-    shape = inputs.shape[:-1] + (cout,)
+    shape = (inputs.size(0), cout) if inputs.dim() == 2 else inputs.shape[:-1] + (cout,)
     if residual is not None:
         _beside(residual, "residual", inputs)
         T.require(residual.shape == shape, "Dense expects (...,cout) residual shape")
