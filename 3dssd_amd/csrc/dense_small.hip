@@ -220,6 +220,11 @@ __device__ __forceinline__ void multiply(f4 (&acc)[NB][NA], const Operand<T, NA>
     }
 }
 
+// The form for up to four steps: there are many such workgroups (a few channels of many points), each no more than a
+// round trip to memory, so what counts is how many a CU holds: five, with 96 registers.  bf16 16384 x 64 x 256: 20 us with
+// two steps ahead (128 registers), 13.6 us with one; fp32 23 and 18.7.  (64 registers spill: 15.6 and 26.)
+constexpr bool few_steps(int na, int nb, int nw) { return na == 2 && nb == 2 && nw == 4; }
+
 constexpr int kSums = 64 * 256;                        // floats of LDS for the waves' sums
 
 // One workgroup's block `pos` of a product, k piece `piece`.  Z: A (ZSIDE 0) or B (ZSIDE 1) is G, and the product takes
@@ -227,8 +232,9 @@ constexpr int kSums = 64 * 256;                        // floats of LDS for the 
 template <class T, bool TA, bool TB, int NA, int NB, int NW, int ZSIDE>
 __device__ __forceinline__ void block_product(const Product &P, unsigned pos, int piece, float *sums) {
     constexpr int E = sizeof(T), kM = 16 * NA, kN = 16 * NB;
-    // steps in flight, by the registers of one
-    constexpr int kSlot = 2 * E * (NA + NB + (ZSIDE == 0 ? NA : ZSIDE == 1 ? NB : 0)), kAhead = kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
+    // steps in flight, by the registers of one; four waves of a 32 x 32 block have one step each
+    constexpr int kSlot = 2 * E * (NA + NB + (ZSIDE == 0 ? NA : ZSIDE == 1 ? NB : 0));
+    constexpr int kAhead = few_steps(NA, NB, NW) ? 1 : kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
     static_assert(NW * kM * kN <= kSums, "the waves' sums");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned nb = (unsigned)((P.N + kN - 1) / kN);
@@ -350,7 +356,7 @@ __device__ __forceinline__ unsigned on_xcd(unsigned b, unsigned blocks) {
 }
 
 template <class T, bool TA, bool TB, int NA, int NB, int NW>
-__global__ __launch_bounds__(NW * 64, NW / 4) void small_kernel(Product P) {
+__global__ __launch_bounds__(NW * 64, few_steps(NA, NB, NW) ? 5 : NW / 4) void small_kernel(Product P) {
     __shared__ __attribute__((aligned(16))) float sums[NW * 256 * NA * NB];
     block_product<T, TA, TB, NA, NB, NW, -1>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
 }
