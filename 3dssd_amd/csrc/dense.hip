@@ -298,7 +298,7 @@ double plan(Plan &L, int type, Kind kind, bool ta, bool tb, long M, long N, long
         for (const auto &t : kShapes) {
             if ((t.shape == kSplit256) != (kind == kSplit)) continue;
             const long c = count(t.m, t.n);
-            for (long s = 1; s == 1 || (s <= 32 && s * 4 <= steps); ++s) {
+            for (long s = 1; s == 1 || (s <= 256 && s * 4 <= steps); s += 1 + s / 16) {
                 const long per = (steps + s - 1) / s, items = c * s, rounds = items / t.slots, rest = items % t.slots;
                 double time = rounds * (per * t.full + t.end);
                 if (rest) time += per * (t.alone + (t.full - t.alone) * rest / t.slots) + t.end;
@@ -345,7 +345,7 @@ int launch_join(int type, const Product &P, hipStream_t s) {
     return SA_OK;
 }
 int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
-    const int rc = L.shape == kSplit256 ? launch_split(L.P, s)
+    const int rc = L.shape == kSplit256 ? launch_split(L.ta, L.P, s)
                                         : launch_tiles(L.shape, type == kF16 ? kF16 : kBF16, type, L.ta, L.tb, L.P, s);
     return rc ? rc : launch_join(type, L.P, s);
 }
@@ -358,6 +358,21 @@ int launch_sums(int type, const float *sums, int strips, int cols, void *out, in
     return SA_OK;
 }
 
+// Takes x (A of a large fp32 product planned on tiles, which would take `time`) as it is, or copied once for its alignment,
+// where that beats its planes: 10 bytes an element, at 4.5 TB/s.
+inline bool split_operand(const Matrix &x) { return x.vec && x.cols % 4 == 0; }
+bool prefer_split(Plan &L, double time, const Matrix &x, bool ta) {
+    const double elements = (double)x.rows * x.cols;
+    Plan split{};
+    const double other = plan(split, kF32, kSplit, ta, true, L.P.M, L.P.N, L.P.K) + (split_operand(x) ? 0 : 8) * elements / 4500;
+    if (!(split_operand(x) || copied_ld(x.cols) < kMaxTileLd / 2) || other >= time + 10 * elements / 4500) return false;
+    L = split;
+    return true;
+}
+void copy_for_split(Jobs &J, int &n, Scratch &ws, Matrix &x) {
+    if (!split_operand(x)) copy_for_tiles(J, n, ws, kF32, x, false);
+}
+
 struct Forward {
     Jobs jobs;
     int njobs;
@@ -367,18 +382,10 @@ void plan_forward(Forward &f, Scratch &ws, int type, long rows, int cin, int cou
     f = Forward{};
     const bool tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w), false);
     const double time = plan(f.plan, type, tiles ? kTiles : kSmall, false, true, rows, cout, cin);
-    if (tiles && type == kF32) {
-        // x as it is, or copied once for its alignment, where that beats its planes (10 bytes an element, at 4.5 TB/s)
-        const bool direct = x.vec && cin % 4 == 0;
-        Plan split{};
-        const double other = plan(split, type, kSplit, false, true, rows, cout, cin);
-        if ((direct || copied_ld(cin) < kMaxTileLd / 2) && other < time + (double)rows * cin * (direct ? 10 : 2) / 4500) {
-            f.plan = split;
-            if (!direct) copy_for_tiles(f.jobs, f.njobs, ws, type, x, false);
-        }
-    }
+    const bool split = tiles && type == kF32 && prefer_split(f.plan, time, x, false);
+    if (split) copy_for_split(f.jobs, f.njobs, ws, x);
     if (tiles) {
-        if (f.plan.shape != kSplit256 && !tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
+        if (!split && !tile_operand(type, x)) copy_for_tiles(f.jobs, f.njobs, ws, type, x);
         if (!tile_operand(type, w)) copy_for_tiles(f.jobs, f.njobs, ws, type, w);
     }
     place(f.plan, ws, x, w);
@@ -422,17 +429,18 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
         j.sums = b.sums = (float *)ws.take((unsigned long)b.strips * cout * 4);
     }
     if (rows && cout && (copy || j.sums)) add_job(b.jobs, b.njobs, j);
-    if (b.tiles && (want & kWantW) && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
-    if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
     const Kind kind = b.tiles ? kTiles : kSmall;
+    if (want & kWantW) {
+        const double time = plan(b.dw, type, kind, true, true, cin, cout, rows);
+        if (b.tiles && type == kF32 && prefer_split(b.dw, time, x, true)) copy_for_split(b.jobs, b.njobs, ws, x);
+        else if (b.tiles && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
+    }
+    if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
     if (want & kWantX) {
         plan(b.dx, type, kind, false, false, rows, cin, cout);
         place(b.dx, ws, d, w);
     }
-    if (want & kWantW) {
-        plan(b.dw, type, kind, true, true, cin, cout, rows);
-        place(b.dw, ws, x, d);
-    }
+    if (want & kWantW) place(b.dw, ws, x, d);
     if (act != kNone && !copy) {
         for (Product *P : {&b.dx.P, &b.dw.P}) {
             P->z = z.p; P->ldz = z.ld; P->vec_z = z.vec; P->zact = act;

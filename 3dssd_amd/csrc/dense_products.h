@@ -13,10 +13,10 @@ constexpr long kMaxTileLd = 1L << 21, kMaxLd = 1L << 24;
 enum TileShape { kNoTile = 0, kTile256 = 1, kTile256x128 = 2, kTile128 = 3, kSplit256 = 4 };
 int launch_tiles(int shape, int type, int out_type, bool ta, bool tb, const Product &P, hipStream_t s);
 
-// A in fp32 (k contiguous, 16-byte aligned base and rows, fewer than kMaxTileLd / 2 elements apart, K a multiple of 4 or
-// zeros behind it up to one), B as three bf16 planes (n contiguous, like the tiles' operands), to fp32, on tiles of 256 x 256; P.passes is 1
-// and P.kchunk counts steps of 32 k.
-int launch_split(const Product &P, hipStream_t s);
+// A in fp32 (k, or with ta m, contiguous; 16-byte aligned base and rows, fewer than kMaxTileLd / 2 elements apart; along the
+// contiguous index a multiple of 4, or zeros behind it up to one), B as three bf16 planes (n contiguous, like the tiles'
+// operands), to fp32, on tiles of 256 x 256; P.passes is 1 and P.kchunk counts steps of 32 k.
+int launch_split(bool ta, const Product &P, hipStream_t s);
 
 // Any forward product (A k-contiguous, B n-contiguous); P.kchunk counts k indices (a multiple of 32).
 int launch_small_forward(int type, const Product &P, hipStream_t s);

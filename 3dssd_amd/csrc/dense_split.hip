@@ -72,6 +72,7 @@ struct Splitting {
     }
 };
 
+template <bool TA>
 __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
     __shared__ __attribute__((aligned(1024))) char lds[9 * kPlane];    // A's planes of two steps, B's of one
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -83,18 +84,19 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
 
     Loader<kEdge, W, true, kK> lb;
     lb.init(wave, lane, P.ldb);
-    Reader<kEdge, false, kK> ra;
+    Reader<kEdge, TA, kK> ra;
     Reader<kEdge, true, kK> rb;
     const int wm = wave % 2 * 128, wn = wave / 2 * 64;
     ra.init(wm, lane);
     rb.init(wn, lane);
-    // A's values on their way: pieces of eight k, number g 512 + thread; four neighbours have one row
-    const int row = threadIdx.x >> 2, key = (threadIdx.x & 3) * 8;
-    const unsigned off = (unsigned)(row * P.lda + key) * 4, put = row * 64 + (((threadIdx.x & 3) ^ piece_of<kK>(row)) * 16);
+    // A's values on their way: pieces of eight along k (m with TA), number g 512 + thread; 4 (32) neighbours have one row (k)
+    const int outer = threadIdx.x / (TA ? 32 : 4), piece = threadIdx.x % (TA ? 32 : 4), key = piece * 8;
+    const unsigned off = (unsigned)(outer * P.lda + key) * 4;
+    const unsigned put = TA ? outer * 512 + (piece ^ 2 * slot_of(outer)) * 16 : outer * 64 + (piece ^ piece_of<kK>(outer)) * 16;
 
     const int per = (int)((P.K + kK - 1) / kK), k_tail = (int)(P.K - (long)(per - 1) * kK);
-    const int step_b = (int)P.ldb * kK * 2;
-    const unsigned inc_a = (unsigned)P.lda * 4 * 128, inc_b = (unsigned)P.ldb * 2 * lb.kStep;
+    const int step_a = (int)(TA ? P.lda : 1) * kK * 4, step_b = (int)P.ldb * kK * 2;
+    const unsigned inc_a = (unsigned)P.lda * 4 * (TA ? 16 : 128), inc_b = (unsigned)P.ldb * 2 * lb.kStep;
     const long plane = P.plane_b * 2;
     unsigned load_item = item;
     int load_left = 0, kstep = 0, kk = 0;
@@ -110,11 +112,12 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
             load_left = p.steps;
             kstep = p.first;
             const int rows_a = R.M - p.m0 < kEdge ? (int)(R.M - p.m0) : kEdge, rows_b = R.N - p.n0 < kEdge ? (int)(R.N - p.n0) : kEdge;
-            full_a = (unsigned)(((rows_a - 1) * R.lda + kK) * 4);
-            tail_a = (unsigned)(((rows_a - 1) * R.lda + round_up(k_tail, 4)) * 4);
+            auto bytes = [&](int k) { return (unsigned)(((TA ? k - 1 : rows_a - 1) * R.lda + (TA ? rows_a : k) + 3) & ~3L) * 4; };
+            full_a = bytes(kK);
+            tail_a = bytes(k_tail);
             full_b = lb.bytes(R.ldb, rows_b, kK);
             tail_b = lb.bytes(R.ldb, rows_b, k_tail);
-            next_a = (const char *)R.a + (p.m0 * R.lda + (long)kstep * kK) * 4;
+            next_a = (const char *)R.a + (TA ? p.m0 : p.m0 * R.lda) * 4 + (long)kstep * step_a;
             next_b = (const char *)R.b + p.n0 * 2 + (long)kstep * step_b;
         }
         const bool some = load_left != 0, last = kstep == per - 1;     // past the last item: zeros, from nowhere
@@ -126,7 +129,7 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
         if (some) {
             --load_left;
             ++kstep;
-            next_a += 4 * kK;
+            next_a += step_a;
             next_b += step_b;
         }
     };
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
         const auto r = __builtin_amdgcn_make_buffer_rsrc((void *)(at_a + g * (long)inc_a), 0, rest > 0 ? rest : 0, 0x00020000);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const u4 v = __builtin_amdgcn_raw_buffer_load_b128(r, key + 4 * h < kk ? off + 16 * h : kOutside, 0, 0);
+            const u4 v = __builtin_amdgcn_raw_buffer_load_b128(r, TA || key + 4 * h < kk ? off + 16 * h : kOutside, 0, 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[g].x[4 * h + c] = __uint_as_float(v[c]);
         }
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
     auto keep_a = [&](int g, unsigned to) __attribute__((always_inline)) {
         s[g].infinities();
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *(lds_w4)(uintptr_t)(to + p * kPlane + g * 128 * 64 + put) = s[g].plane[p];
+        for (int p = 0; p < 3; ++p) *(lds_w4)(uintptr_t)(to + p * kPlane + g * (kPlane / 2) + put) = s[g].plane[p];
     };
     constexpr int LB = lb.kLoads;
     auto load_b = [&](int q) __attribute__((always_inline)) {
@@ -232,10 +235,12 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
 
 }  // namespace
 
-int dense::launch_split(const Product &P, hipStream_t s) {
+int dense::launch_split(bool ta, const Product &P, hipStream_t s) {
     const long items = ((P.M + kEdge - 1) / kEdge) * ((P.N + kEdge - 1) / kEdge) * P.splits;
     if (items > 0x3fffffffL) return SA_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(split_kernel, dim3((unsigned)(items < 256 ? items : 256)), dim3(W * 64), 0, s, P);
+    const dim3 grid((unsigned)(items < 256 ? items : 256));
+    if (ta) hipLaunchKernelGGL(split_kernel<true>, grid, dim3(W * 64), 0, s, P);
+    else hipLaunchKernelGGL(split_kernel<false>, grid, dim3(W * 64), 0, s, P);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }

@@ -204,6 +204,11 @@ def test_large_fp32_products_at_odd_places(gpu, size, pad):
     plain = m.dense(x, w)
     _check_forward(x, w, None, None, None, plain, None)
     assert torch.equal(m.dense(x, w), plain)
+    g = _rand(gpu, (rows, cout), torch.float32, i + 4, 0.05)
+    for act in ("silu", None):
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=pre if act else None)
+        _check_grad(x, w, g, act, pre, dx, dw, db)
+        assert torch.equal(m.dense_grad(x, w, g, activation=act, preact=pre, needs=(False, True))[1], dw)
 
 
 @pytest.mark.gpu
