@@ -20,16 +20,31 @@ __device__ __forceinline__ Eight<T> fetch(const T *row, int c, int cols) {
     return v;
 }
 
-// The pieces of a split k range, summed in piece order, then the epilogue.
-template <class T>
+// The pieces of a split k range, summed in a fixed order, then the epilogue.  G groups of threads share the pieces of the same
+// sums where there are many pieces and few sums (128 x 256 sums of 228 pieces: 7.5 us with 8 groups, 14 with one).
+template <class T, int G>
 __global__ __launch_bounds__(256) void join_kernel(Product P) {
+    constexpr int kOwn = 256 / G;
+    __shared__ f4 part[G][kOwn];
+    const int own = threadIdx.x % kOwn, group = threadIdx.x / kOwn;
     const long Np = round_up(P.N, 4), per = Np / 4, total = P.M * per, plane = P.M * Np;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long m = i / per, n = (i - m * per) * 4;
-        const float *p = P.part + m * Np + n;
-        f4 s = *(const f4 *)p;
+    for (long i0 = (long)blockIdx.x * kOwn; i0 < total; i0 += (long)gridDim.x * kOwn) {
+        const long i = i0 + own, m = i / per, n = (i - m * per) * 4;
+        const float *p = P.part + (long)group * plane + m * Np + n;
+        f4 s{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < total) {
+            if (group < P.splits) s = *(const f4 *)p;
 #pragma unroll 8
-        for (int z = 1; z < P.splits; ++z) s += *(const f4 *)(p + z * plane);
+            for (int z = group + G; z < P.splits; z += G) s += *(const f4 *)(p + (z - group) * plane);
+        }
+        if constexpr (G > 1) {
+            __syncthreads();
+            part[group][own] = s;
+            __syncthreads();
+#pragma unroll
+            for (int g = 1; g < G; ++g) s += part[g][own];
+        }
+        if (group != 0 || i >= total) continue;
         float b[4];
         load_bias<T, 4>(P.e, n, P.N, b);
         const float v[4] = {s[0], s[1], s[2], s[3]};
@@ -174,17 +189,20 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void sum_strips_kernel(const float *sums, int strips, int cols, T *out) {
-    __shared__ float part[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void sum_strips_kernel(const float *sums, int strips, int cols, T *out) {
+    __shared__ float part[16][64];
+    const int own = threadIdx.x & 63, c = blockIdx.x * 64 + own, q = threadIdx.x >> 6;
     float s = 0.0f;
     if (c < cols) {
 #pragma unroll 8
-        for (int i = q; i < strips; i += 4) s += sums[(long)i * cols + c];
+        for (int i = q; i < strips; i += 16) s += sums[(long)i * cols + c];
     }
-    part[q][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (q == 0 && c < cols) out[c] = from_f32<T>((part[0][c & 63] + part[1][c & 63]) + (part[2][c & 63] + part[3][c & 63]));
+    part[q][own] = s;
+    for (int half = 8; half >= 1; half /= 2) {
+        __syncthreads();
+        if (q < half) part[q][own] += part[q + half][own];
+    }
+    if (q == 0 && c < cols) out[c] = from_f32<T>(part[0][own]);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -334,15 +352,19 @@ void place(Plan &L, Scratch &ws, const Matrix &a, const Matrix &b) {
     P.part = P.splits > 1 ? (float *)ws.take((unsigned long)P.splits * P.M * round_up(P.N, 4) * 4) : nullptr;
 }
 
+template <int G>
 int launch_join(int type, const Product &P, hipStream_t s) {
-    if (P.splits == 1) return SA_OK;
-    const long n = (P.M * (round_up(P.N, 4) / 4) + 255) / 256;
+    const long n = (P.M * (round_up(P.N, 4) / 4) + 256 / G - 1) / (256 / G);
     const dim3 blocks((unsigned)(n < 8192 ? n : 8192));
-    if (type == kF32) hipLaunchKernelGGL((join_kernel<float>), blocks, dim3(256), 0, s, P);
-    else if (type == kBF16) hipLaunchKernelGGL((join_kernel<bf16_t>), blocks, dim3(256), 0, s, P);
-    else hipLaunchKernelGGL((join_kernel<f16_t>), blocks, dim3(256), 0, s, P);
+    if (type == kF32) hipLaunchKernelGGL((join_kernel<float, G>), blocks, dim3(256), 0, s, P);
+    else if (type == kBF16) hipLaunchKernelGGL((join_kernel<bf16_t, G>), blocks, dim3(256), 0, s, P);
+    else hipLaunchKernelGGL((join_kernel<f16_t, G>), blocks, dim3(256), 0, s, P);
     SA_CHECK_LAUNCH();
     return SA_OK;
+}
+int launch_join(int type, const Product &P, hipStream_t s) {
+    if (P.splits == 1) return SA_OK;
+    return P.splits >= 32 && P.M * P.N <= 1L << 17 ? launch_join<8>(type, P, s) : launch_join<1>(type, P, s);
 }
 int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
     const int rc = L.shape == kSplit256 ? launch_split(L.ta, L.P, s)
@@ -351,9 +373,9 @@ int launch_tile_plan(int type, const Plan &L, hipStream_t s) {
 }
 int launch_sums(int type, const float *sums, int strips, int cols, void *out, int out_f32, hipStream_t s) {
     const dim3 grid((cols + 63) / 64);
-    if (out_f32 || type == kF32) hipLaunchKernelGGL((sum_strips_kernel<float>), grid, dim3(256), 0, s, sums, strips, cols, (float *)out);
-    else if (type == kBF16) hipLaunchKernelGGL((sum_strips_kernel<bf16_t>), grid, dim3(256), 0, s, sums, strips, cols, (bf16_t *)out);
-    else hipLaunchKernelGGL((sum_strips_kernel<f16_t>), grid, dim3(256), 0, s, sums, strips, cols, (f16_t *)out);
+    if (out_f32 || type == kF32) hipLaunchKernelGGL((sum_strips_kernel<float>), grid, dim3(1024), 0, s, sums, strips, cols, (float *)out);
+    else if (type == kBF16) hipLaunchKernelGGL((sum_strips_kernel<bf16_t>), grid, dim3(1024), 0, s, sums, strips, cols, (bf16_t *)out);
+    else hipLaunchKernelGGL((sum_strips_kernel<f16_t>), grid, dim3(1024), 0, s, sums, strips, cols, (f16_t *)out);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
