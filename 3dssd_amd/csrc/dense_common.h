@@ -214,6 +214,7 @@ struct Product {
     long plane_a, plane_b;   // elements between planes
     float *part;          // splits > 1: [splits][M][Np] partial sums, Np = N rounded up to a multiple of 4
     Epilogue e;
+    int alone;            // small products: a block for each wave of a workgroup
     // small backward products
     const void *z;        // operand G becomes G act'(z), or null
     long ldz;

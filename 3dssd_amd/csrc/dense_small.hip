@@ -227,7 +227,20 @@ constexpr bool few_steps(int na, int nb, int nw) { return na == 2 && nb == 2 && 
 
 constexpr int kSums = 64 * 256;                        // floats of LDS for the waves' sums
 
-// One workgroup's block `pos` of a product, k piece `piece`.  Z: A (ZSIDE 0) or B (ZSIDE 1) is G, and the product takes
+// The waves of a block wait for each other; one alone needs its own LDS accesses in order only (and has no partners: the other
+// waves of its workgroup may be done).
+template <int NW>
+__device__ __forceinline__ void meet() {
+    if constexpr (NW > 1) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Block `pos` of a product, k piece `piece`, by NW neighbouring waves, with `sums` for them alone; the workgroup's other waves do
+// the same with blocks of their own, or beyond the last.  Z: A (ZSIDE 0) or B (ZSIDE 1) is G, and the product takes
 // G act'(Z) with Z = P.z in G's place (rows of P.ldz).
 template <class T, bool TA, bool TB, int NA, int NB, int NW, int ZSIDE>
 __device__ __forceinline__ void block_product(const Product &P, unsigned pos, int piece, float *sums) {
@@ -236,7 +249,7 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
     constexpr int kSlot = 2 * E * (NA + NB + (ZSIDE == 0 ? NA : ZSIDE == 1 ? NB : 0));
     constexpr int kAhead = few_steps(NA, NB, NW) ? 1 : kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
     static_assert(NW * kM * kN <= kSums, "the waves' sums");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int thread = threadIdx.x % (NW * 64), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const unsigned nb = (unsigned)((P.N + kN - 1) / kN);
     const long m0 = (long)(pos / nb) * kM, n0 = (long)(pos % nb) * kN;
     const long k0 = (long)piece * P.kchunk, kend = k0 + P.kchunk < P.K ? k0 + P.kchunk : P.K;
@@ -264,7 +277,7 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
     typename SA::Regs ra[kAhead];
     typename SB::Regs rb[kAhead];
     typename SZ::Regs rz[ZSIDE >= 0 ? kAhead : 1];
-    const long steps = (kend - k0 + 31) / 32;
+    const long steps = m0 < P.M ? (kend - k0 + 31) / 32 : 0;
     auto fetch = [&](int slot, long s) {
         const long l = kend - k0 - s * 32;
         const int left = l < 32 ? (int)l : 32;
@@ -308,11 +321,11 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 sums[(wave * kM + SA::row(x, lane & 15)) * kN + SB::row(y, 4 * (lane >> 4) + r)] = acc[y][x][r];
-    __syncthreads();
+    meet<NW>();
     const long Np = round_up(P.N, 4);
     const int used = steps < NW ? (int)steps : NW;     // the others' sums are zero
 #pragma unroll 1
-    for (int q = threadIdx.x; q < kM * kN / 4; q += NW * 64) {
+    for (int q = thread; q < kM * kN / 4; q += NW * 64) {
         const int lm = q / (kN / 4), ln = q % (kN / 4) * 4;
         const long m = m0 + lm, n = n0 + ln;
         if (m >= P.M || n >= P.N) continue;
@@ -333,15 +346,15 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
         }
     }
     if (summed) {                                      // four k groups of NW waves for each column
-        __syncthreads();
+        meet<NW>();
 #pragma unroll
         for (int t = 0; t < NB; ++t) sums[(wave * 4 + (lane >> 4)) * kN + SB::row(t, lane & 15)] = column[t];
-        __syncthreads();
-        const long n = n0 + threadIdx.x;
-        if (threadIdx.x < kN && n < P.N) {
+        meet<NW>();
+        const long n = n0 + thread;
+        if (thread < kN && n < P.N) {
             float v = 0.0f;
 #pragma unroll 8
-            for (int w = 0; w < 4 * NW; ++w) v += sums[w * kN + threadIdx.x];
+            for (int w = 0; w < 4 * NW; ++w) v += sums[w * kN + thread];
             if (P.splits > 1) P.colpart[(long)piece * P.N + n] = v;
             else if (P.col_f32) ((float *)P.colsum)[n] = v;
             else ((T *)P.colsum)[n] = from_f32<T>(v);
@@ -361,21 +374,49 @@ __global__ __launch_bounds__(NW * 64, few_steps(NA, NB, NW) ? 5 : NW / 4) void s
     block_product<T, TA, TB, NA, NB, NW, -1>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
 }
 
-// dX and dW of a layer in one launch: the first `nw` workgroups are dW's (all blocks of a piece, then the next piece), the
-// others dX's.  dW's blocks have WT x WT MFMA tiles.  128 registers: two workgroups of eight waves per CU.
-template <class T, bool Z, int WT, int NW>
-__global__ __launch_bounds__(NW * 64, 4) void small_backward_kernel(Product X, Product W, unsigned nw) {
-    __shared__ __attribute__((aligned(16))) float sums[NW * 1024];
-    if (blockIdx.x < nw) {
-        const unsigned blocks = nw / W.splits;
-        block_product<T, true, true, WT, WT, NW, Z ? 1 : -1>(W, on_xcd(blockIdx.x % blocks, blocks), blockIdx.x / blocks, sums);
+// A workgroup's share of a product: block `group`, or with P.alone (ALONE: which may be set) a block for each of its waves.
+template <class T, bool TA, bool TB, int WT, int NW, int ZSIDE, bool ALONE>
+__device__ __forceinline__ void group_product(const Product &P, unsigned group, int piece, float *sums) {
+    if (!ALONE || !P.alone) {
+        block_product<T, TA, TB, WT, WT, NW, ZSIDE>(P, group, piece, sums);
     } else {
-        const unsigned b = blockIdx.x - nw, blocks = (gridDim.x - nw) / X.splits;
-        block_product<T, false, false, 2, 2, NW, Z ? 0 : -1>(X, on_xcd(b % blocks, blocks), b / blocks, sums);
+        const unsigned mine = threadIdx.x >> 6;
+        block_product<T, TA, TB, WT, WT, 1, ZSIDE>(P, group * NW + mine, piece, sums + mine * (256 * WT * WT));
+    }
+}
+
+// dX and dW of a layer in one launch: the workgroups from x0 to x1 are dX's (all blocks of a piece, then the next piece), the
+// others, in front of those or behind, dW's.  dW's blocks have WT x WT MFMA tiles.  128 registers: two workgroups of eight
+// waves per CU.
+template <class T, bool Z, int WT, int NW, bool ALONE>
+__global__ __launch_bounds__(NW * 64, 4) void small_backward_kernel(Product X, Product W, unsigned x0, unsigned x1) {
+    __shared__ __attribute__((aligned(16))) float sums[NW * 1024];
+    if (blockIdx.x < x0 || blockIdx.x >= x1) {
+        const unsigned b = blockIdx.x < x0 ? blockIdx.x : blockIdx.x - x1, groups = (gridDim.x - (x1 - x0)) / W.splits;
+        group_product<T, true, true, WT, NW, Z ? 1 : -1, ALONE>(W, on_xcd(b % groups, groups), b / groups, sums);
+    } else {
+        const unsigned b = blockIdx.x - x0, groups = (x1 - x0) / X.splits;
+        group_product<T, false, false, 2, NW, Z ? 0 : -1, ALONE>(X, on_xcd(b % groups, groups), b / groups, sums);
     }
 }
 
 inline long blocks_of(const Product &P, long m, long n) { return ((P.M + m - 1) / m) * ((P.N + n - 1) / n); }
+
+// four blocks of 32 x 32 for as many waves
+template <class T>
+__global__ __launch_bounds__(256, 4) void small_alone_kernel(Product P) {
+    __shared__ __attribute__((aligned(16))) float sums[4 * 1024];
+    group_product<T, false, true, 2, 4, -1, true>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
+}
+template <class T>
+int launch_alone(Product P, hipStream_t s) {
+    P.alone = 1;
+    const long groups = (blocks_of(P, 32, 32) + 3) / 4;
+    if (groups > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((small_alone_kernel<T>), dim3((unsigned)groups, P.splits), dim3(256), 0, s, P);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
 
 template <class T, bool TA, bool TB, int NA, int NB, int NW>
 int launch(const Product &P, hipStream_t s) {
@@ -398,6 +439,7 @@ int launch_forward(Product P, hipStream_t s) {
     if (P.M > 32 || (P.M > 16 && !can(4))) {
         // blocks of 32 x 32; four waves suffice for four steps
         P.vec_b = whole(P.b, P.ldb, P.N, 2, E);
+        if (P.kchunk <= (E == 4 ? 32 : 64) && blocks_of(P, 32, 32) >= 2048) return launch_alone<T>(P, s);
         return P.kchunk <= 128 ? launch<T, false, true, 2, 2, 4>(P, s) : launch<T, false, true, 2, 2, 16>(P, s);
     }
     // few rows: as many columns per lane as the alignment allows and as still leave 128 workgroups
@@ -414,9 +456,23 @@ int launch_forward(Product P, hipStream_t s) {
     return launch<T, false, true, 1, 1, 16>(P, s);
 }
 
+// nx, nw: blocks of a piece
 template <class T, bool Z, int WT, int NW>
-int launch_backward(const Product &X, const Product &W, long nx, long nw, hipStream_t s) {
-    hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW>), dim3((unsigned)(nx + nw)), dim3(NW * 64), 0, s, X, W, (unsigned)nw);
+int launch_backward(Product X, Product W, long nx, long nw, hipStream_t s) {
+    // One wave's steps are few where a layer is narrow on one side, and the product on that side all output: fp32 6 x 3217 x
+    // 16023, whose dW is 200 MB of sums of six terms, takes 190 us instead of 412.  (With a few workgroups only, the waves
+    // share the work of a block as elsewhere.  No rule looks at the other product: the order of a sum does not depend on it.)
+    auto groups = [](Product &P, long blocks) {
+        P.alone = P.kchunk <= 64 && blocks * P.splits >= 2048;
+        return (P.alone ? (blocks + NW - 1) / NW : blocks) * P.splits;
+    };
+    const long gx = groups(X, nx), gw = groups(W, nw), x0 = X.kchunk > W.kchunk ? 0 : gw;      // the longer ones first
+    if (gx + gw > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(gx + gw)), block(NW * 64);
+    if (X.alone || W.alone)
+        hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, true>), grid, block, 0, s, X, W, (unsigned)x0, (unsigned)(x0 + gx));
+    else
+        hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, false>), grid, block, 0, s, X, W, (unsigned)x0, (unsigned)(x0 + gx));
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
@@ -428,9 +484,8 @@ int launch_backward(const Product &X, Product W, long nx, bool z, hipStream_t s)
         W.vec_a = whole(W.a, W.lda, W.M, WT, E);
         W.vec_b = whole(W.b, W.ldb, W.N, WT, E);
         W.vec_z = W.z && whole(W.z, W.ldz, W.N, WT, E);
-        nw = blocks_of(W, 16 * WT, 16 * WT) * W.splits;
+        nw = blocks_of(W, 16 * WT, 16 * WT);
     }
-    if (nx + nw > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
     const bool shorter = (nx == 0 || X.kchunk <= 128) && (nw == 0 || W.kchunk <= 128);
     if (z) return shorter ? launch_backward<T, true, WT, 4>(X, W, nx, nw, s) : launch_backward<T, true, WT, 8>(X, W, nx, nw, s);
     return shorter ? launch_backward<T, false, WT, 4>(X, W, nx, nw, s) : launch_backward<T, false, WT, 8>(X, W, nx, nw, s);
@@ -441,7 +496,7 @@ int launch_backward(const Product *px, const Product *pw, hipStream_t s) {
     X.splits = W.splits = 1;
     if (px) X = *px;
     if (pw) W = *pw;
-    const long nx = px ? blocks_of(X, 32, 32) * X.splits : 0;
+    const long nx = px ? blocks_of(X, 32, 32) : 0;
     const bool z = X.z || W.z;
     // fp32 products take a CU long (16 x 16 x 4 per MFMA of 32 cycles): smaller blocks where there are few
     if constexpr (sizeof(T) == 4)

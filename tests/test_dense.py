@@ -119,7 +119,9 @@ SIZES = [(1, 1, 1), (1, 64, 8), (1, 1027, 515), (3, 5, 7), (17, 67, 33), (64, 64
          (2048, 512, 128), (1, 4096, 1024), (8, 1024, 1000), (16, 640, 512), (31, 1000, 2048), (4099, 40, 72),
          # products of the tile kernel: its edges, odd operands (copied first), many and few tiles, short and long k
          (640, 520, 648), (33, 8192, 520), (129, 1030, 2056), (3585, 72, 3400), (2049, 2065, 33), (70001, 40, 33), (384, 4096, 256),
-         (4100, 72, 4104), (8200, 136, 1032), (1100, 1100, 1100), (30001, 264, 520), (520, 30001, 136), (2050, 1027, 1030)]
+         (4100, 72, 4104), (8200, 136, 1032), (1100, 1100, 1100), (30001, 264, 520), (520, 30001, 136), (2050, 1027, 1030),
+         # narrow on one side: products of few steps, with and without a bias in them
+         (7, 3217, 1603), (24, 1862, 1394), (12501, 265, 8), (16389, 8, 517), (65, 2051, 1112), (64, 2048, 1153)]
 
 
 # ------------------------------------------------------------------------------------------------------- CPU: refusals
