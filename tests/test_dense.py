@@ -533,3 +533,31 @@ def test_a_training_step_of_a_residual_block(gpu, dt):
     assert abs(float(norm) - ref) <= tol * ref and ref > 5.0
     for got, want, what in zip(clipped, grads[1:], ("w1", "b1", "w2", "b2")):
         close(got, want * (5.0 / ref), what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", [(1, 64, 8), (129, 257, 130), (2048, 512, 128), (1100, 1100, 1100), (5003, 771, 1283)])
+def test_slopes_kept_in_32_bits(gpu, dt, size):
+    """round_slopes=False: no rounding of grad_out * slope, so what is left are the fp32 sums and one rounding per result."""
+    m = _mod()
+    rows, cin, cout = size
+    for i, act in enumerate(ACTS):
+        x, w = _rand(gpu, (rows, cin), dt, i), _rand(gpu, (cin, cout), dt, 10 + i, math.sqrt(2.0 / cin))
+        g, z = _rand(gpu, (rows, cout), dt, 20 + i, 0.05), _rand(gpu, (rows, cout), dt, 30 + i)
+        b = torch.empty(cout, dtype=(dt, torch.float32)[i % 2], device=gpu)
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z, round_slopes=False)
+        assert dx.dtype == dw.dtype == dt and db.dtype == b.dtype
+        d = g.double() * _slope64(z.double(), act)
+        dd = 0 * d if act is None else 32 * U * g.double().abs() * (1 + z.double().abs()) + _tiny(torch.float32)
+        wt, xt = w.double().t().contiguous(), x.double().t().contiguous()
+        for got, want, bound, what in (
+                (dx, d @ wt, (_sum_bound(cout) * (d.abs() + dd) + dd) @ wt.abs(), "grad_inputs"),
+                (dw, xt @ d, xt.abs() @ (_sum_bound(rows) * (d.abs() + dd) + dd), "grad_weights"),
+                (db, d.sum(0), (_sum_bound(rows) * (d.abs() + dd) + dd).sum(0), "grad_biases")):
+            _within(got, want, _half(got.dtype) * (want.abs() + bound) + bound + _tiny(got.dtype), what)
+        only = m.dense_grad(x, w, g, activation=act, preact=z, needs=(False, True), round_slopes=False)
+        assert only[0] is None and torch.equal(only[1], dw) and only[2] is None
+        if dt == torch.float32 or act is None:         # nothing is rounded there either way
+            for a, b_ in zip((dx, dw, db), m.dense_grad(x, w, g, biases=b, activation=act, preact=z)):
+                assert torch.equal(a, b_)
