@@ -215,6 +215,7 @@ struct Product {
     float *part;          // splits > 1: [splits][M][Np] partial sums, Np = N rounded up to a multiple of 4
     Epilogue e;
     int alone;            // small products: a block for each wave of a workgroup
+    unsigned first;       // small products: the first block, or group of `alone` blocks, of this launch
     // small backward products
     const void *z;        // operand G becomes G act'(z), or null
     long ldz;

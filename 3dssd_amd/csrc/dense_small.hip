@@ -371,7 +371,7 @@ __device__ __forceinline__ unsigned on_xcd(unsigned b, unsigned blocks) {
 template <class T, bool TA, bool TB, int NA, int NB, int NW>
 __global__ __launch_bounds__(NW * 64, few_steps(NA, NB, NW) ? 5 : NW / 4) void small_kernel(Product P) {
     __shared__ __attribute__((aligned(16))) float sums[NW * 256 * NA * NB];
-    block_product<T, TA, TB, NA, NB, NW, -1>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
+    block_product<T, TA, TB, NA, NB, NW, -1>(P, P.first + on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
 }
 
 // A workgroup's share of a product: block `group`, or with P.alone (ALONE: which may be set) a block for each of its waves.
@@ -393,38 +393,49 @@ __global__ __launch_bounds__(NW * 64, 4) void small_backward_kernel(Product X, P
     __shared__ __attribute__((aligned(16))) float sums[NW * 1024];
     if (blockIdx.x < x0 || blockIdx.x >= x1) {
         const unsigned b = blockIdx.x < x0 ? blockIdx.x : blockIdx.x - x1, groups = (gridDim.x - (x1 - x0)) / W.splits;
-        group_product<T, true, true, WT, NW, Z ? 1 : -1, ALONE>(W, on_xcd(b % groups, groups), b / groups, sums);
+        group_product<T, true, true, WT, NW, Z ? 1 : -1, ALONE>(W, W.first + on_xcd(b % groups, groups), b / groups, sums);
     } else {
         const unsigned b = blockIdx.x - x0, groups = (x1 - x0) / X.splits;
-        group_product<T, false, false, 2, NW, Z ? 0 : -1, ALONE>(X, on_xcd(b % groups, groups), b / groups, sums);
+        group_product<T, false, false, 2, NW, Z ? 0 : -1, ALONE>(X, X.first + on_xcd(b % groups, groups), b / groups, sums);
     }
 }
 
 inline long blocks_of(const Product &P, long m, long n) { return ((P.M + m - 1) / m) * ((P.N + n - 1) / n); }
 
+// A grid ends at 2^32 work items -- beyond, it is cut off without an error -- and a narrow layer of 2^27 rows has more: then the
+// blocks go in several launches.  (A k range is only split where there are fewer blocks than CUs.)
+inline long most(long threads) { return (1L << 31) / threads; }
+template <class F>
+int in_launches(long blocks, long threads, F &&one) {
+    if (blocks > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
+    for (long at = 0; at < blocks; at += most(threads)) {
+        one((unsigned)at, (unsigned)(blocks - at < most(threads) ? blocks - at : most(threads)));
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
 // four blocks of 32 x 32 for as many waves
 template <class T>
 __global__ __launch_bounds__(256, 4) void small_alone_kernel(Product P) {
     __shared__ __attribute__((aligned(16))) float sums[4 * 1024];
-    group_product<T, false, true, 2, 4, -1, true>(P, on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
+    group_product<T, false, true, 2, 4, -1, true>(P, P.first + on_xcd(blockIdx.x, gridDim.x), blockIdx.y, sums);
 }
 template <class T>
 int launch_alone(Product P, hipStream_t s) {
     P.alone = 1;
-    const long groups = (blocks_of(P, 32, 32) + 3) / 4;
-    if (groups > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((small_alone_kernel<T>), dim3((unsigned)groups, P.splits), dim3(256), 0, s, P);
-    SA_CHECK_LAUNCH();
-    return SA_OK;
+    return in_launches((blocks_of(P, 32, 32) + 3) / 4, 256, [&](unsigned first, unsigned groups) {
+        P.first = first;
+        hipLaunchKernelGGL((small_alone_kernel<T>), dim3(groups, P.splits), dim3(256), 0, s, P);
+    });
 }
 
 template <class T, bool TA, bool TB, int NA, int NB, int NW>
-int launch(const Product &P, hipStream_t s) {
-    const long blocks = blocks_of(P, 16 * NA, 16 * NB);
-    if (blocks > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((small_kernel<T, TA, TB, NA, NB, NW>), dim3((unsigned)blocks, P.splits), dim3(NW * 64), 0, s, P);
-    SA_CHECK_LAUNCH();
-    return SA_OK;
+int launch(Product P, hipStream_t s) {
+    return in_launches(blocks_of(P, 16 * NA, 16 * NB), NW * 64, [&](unsigned first, unsigned blocks) {
+        P.first = first;
+        hipLaunchKernelGGL((small_kernel<T, TA, TB, NA, NB, NW>), dim3(blocks, P.splits), dim3(NW * 64), 0, s, P);
+    });
 }
 
 // pieces of c rows of an operand with rows contiguous: aligned, and no parts of them
@@ -467,14 +478,24 @@ int launch_backward(Product X, Product W, long nx, long nw, hipStream_t s) {
         return (P.alone ? (blocks + NW - 1) / NW : blocks) * P.splits;
     };
     const long gx = groups(X, nx), gw = groups(W, nw), x0 = X.kchunk > W.kchunk ? 0 : gw;      // the longer ones first
-    if (gx + gw > 0x7fffffffL) return SA_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)(gx + gw)), block(NW * 64);
-    if (X.alone || W.alone)
-        hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, true>), grid, block, 0, s, X, W, (unsigned)x0, (unsigned)(x0 + gx));
-    else
-        hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, false>), grid, block, 0, s, X, W, (unsigned)x0, (unsigned)(x0 + gx));
-    SA_CHECK_LAUNCH();
-    return SA_OK;
+    const dim3 block(NW * 64);
+    auto launch = [&](unsigned blocks, unsigned x0, unsigned x1) {
+        if (X.alone || W.alone) hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, true>), dim3(blocks), block, 0, s, X, W, x0, x1);
+        else hipLaunchKernelGGL((small_backward_kernel<T, Z, WT, NW, false>), dim3(blocks), block, 0, s, X, W, x0, x1);
+    };
+    if (gx + gw <= most(NW * 64)) {
+        launch((unsigned)(gx + gw), (unsigned)x0, (unsigned)(x0 + gx));
+        SA_CHECK_LAUNCH();
+        return SA_OK;
+    }
+    const int rc = in_launches(gx, NW * 64, [&](unsigned first, unsigned blocks) {
+        X.first = first;
+        launch(blocks, 0, blocks);
+    });
+    return rc ? rc : in_launches(gw, NW * 64, [&](unsigned first, unsigned blocks) {
+        W.first = first;
+        launch(blocks, 0, 0);
+    });
 }
 template <class T, int WT>
 int launch_backward(const Product &X, Product W, long nx, bool z, hipStream_t s) {

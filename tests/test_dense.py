@@ -561,3 +561,44 @@ def test_slopes_kept_in_32_bits(gpu, dt, size):
         if dt == torch.float32 or act is None:         # nothing is rounded there either way
             for a, b_ in zip((dx, dw, db), m.dense_grad(x, w, g, biases=b, activation=act, preact=z)):
                 assert torch.equal(a, b_)
+
+
+@pytest.mark.gpu
+def test_more_work_items_than_a_grid_has(gpu):
+    """Grids end at 2^32 work items: narrow layers of very many rows, and weight gradients of very many elements, have more.
+    What lies behind the first launch's share is looked at, and the first rows."""
+    m = _mod()
+    dt = torch.bfloat16
+
+    def ends(t, rows):
+        return torch.cat([t[:100], t[rows // 2 - 50:rows // 2 + 50], t[-100:]])
+
+    # forward: blocks of 32 rows by sixteen waves
+    rows, cin = (1 << 27) + 70, 136
+    x, w = torch.zeros(rows, cin, dtype=dt, device=gpu), _rand(gpu, (cin, 3), dt, 1)
+    for i, at in enumerate((0, rows // 2 - 50, rows - 100)):
+        x[at:at + 100] = _rand(gpu, (100, cin), dt, 10 + i)
+    out = m.dense(x, w)
+    _check_forward(ends(x, rows), w, None, None, None, ends(out, rows), None)
+    assert not bool(out[100:rows // 2 - 50].any()) and not bool(out[rows // 2 + 50:-100].any())
+    del x, out
+    torch.cuda.empty_cache()
+    # grad_inputs: blocks of 32 rows by eight waves, grad_weights in front or behind
+    rows, cout = (1 << 28) + 70, 72
+    x, w = torch.zeros(rows, 3, dtype=dt, device=gpu), _rand(gpu, (3, cout), dt, 2)
+    g = torch.zeros(rows, cout, dtype=dt, device=gpu)
+    for i, at in enumerate((0, rows // 2 - 50, rows - 100)):
+        g[at:at + 100], x[at:at + 100] = _rand(gpu, (100, cout), dt, 20 + i), _rand(gpu, (100, 3), dt, 30 + i)
+    dx, dw, db = m.dense_grad(x, w, g, biases=torch.empty(cout, device=gpu))
+    _check_grad(ends(x, rows), w, ends(g, rows), None, None, ends(dx, rows), dw, db)
+    assert not bool(dx[100:rows // 2 - 50].any()) and not bool(dx[rows // 2 + 50:-100].any())
+    only = m.dense_grad(x, w, g, needs=(True, False))[0]
+    assert torch.equal(only, dx)
+    del x, g, dx, only
+    torch.cuda.empty_cache()
+    # grad_weights: 2^34 elements and more
+    rows, cin, cout = 72, (1 << 17) + 40, 1 << 17
+    x, g = _rand(gpu, (rows, cin), torch.float32, 3), _rand(gpu, (rows, cout), torch.float32, 4)
+    _, dw, _ = m.dense_grad(x, torch.empty(cin, cout, device=gpu), g, needs=(False, True))
+    for at in (0, cin // 2 - 20, cin - 40):
+        _check_grad(x[:, at:at + 40].contiguous(), g, g, None, None, None, dw[at:at + 40], None)
