@@ -90,23 +90,25 @@ __device__ __forceinline__ void with_activation(int act, F &&f) {
         default: return f(Tag<kNone>{});
     }
 }
-// g act'(z).  ReLU selects: what a closed unit receives, infinities among it, does not come through.
+// g act'(z).  ReLU selects: what a closed unit receives, infinities among it, does not come through.  An infinite z has the slope
+// 0 or 1 (a fp16 z is kept as an infinity from 65520 on, where the forward pass had a finite one): past |z| = 14, 12 or 110 the
+// integral or the logistic is 0 or 1 to every bit, and the product beside it, in which z may be infinite and the other factor
+// 0, is left out.
 template <int ACT>
 __device__ __forceinline__ float times_slope(float g, float z) {
     if constexpr (ACT == kRelu) return z > 0.0f ? g : (z != z ? z : 0.0f);
     if constexpr (ACT == kGelu) {
         float bell;
-        const float tail = normal_tail(z, bell);
-        return g * fmaf(z * 0.39894228040143268f, bell, z >= 0.0f ? 1.0f - tail : tail);
+        const float tail = normal_tail(z, bell), p = z >= 0.0f ? 1.0f - tail : tail;
+        return g * (fabsf(z) > 14.0f ? p : fmaf(z * 0.39894228040143268f, bell, p));
     }
     if constexpr (ACT == kGeluTanh) {
         const float s = logistic(kGeluC * (z + kGeluA * z * z * z));
-        // past |z| = 12 the logistic is 0 or 1 to every bit and the product below would be 0 times infinity
         return g * (fabsf(z) > 12.0f ? s : s + z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
     }
     if constexpr (ACT == kSilu) {
         const float s = logistic(z);
-        return g * (s + z * s * (1.0f - s));
+        return g * (fabsf(z) > 110.0f ? s : s + z * s * (1.0f - s));
     }
     return g;
 }

@@ -602,3 +602,43 @@ def test_more_work_items_than_a_grid_has(gpu):
     _, dw, _ = m.dense_grad(x, torch.empty(cin, cout, device=gpu), g, needs=(False, True))
     for at in (0, cin // 2 - 20, cin - 40):
         _check_grad(x[:, at:at + 40].contiguous(), g, g, None, None, None, dw[at:at + 40], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("size", [(3, 64, 40), (300, 100, 260), (600, 500, 400), (1100, 1100, 1100), (1200, 1104, 1112)])
+def test_slopes_at_infinite_preactivations(gpu, size, act, dt):
+    """The slope is 0 at -infinity and 1 at +infinity, in every kernel that forms one.  (The oracle takes z = -+60 there, where
+    the slopes are 0 and 1 to more than 64 bits' worth of fp32.)"""
+    m = _mod()
+    rows, cin, cout = size
+    x, w = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2, cin ** -0.5)
+    g, z = _rand(gpu, (rows, cout), dt, 3), _rand(gpu, (rows, cout), dt, 4)
+    inf = float("inf")
+    z[0, ::3], z[0, 1::3], z[rows - 1, cout - 1], z[rows // 2, 0] = inf, -inf, -inf, inf
+    finite = z.clamp(-60, 60)
+    b = torch.empty(cout, dtype=torch.float32, device=gpu)
+    _check_grad(x, w, g, act, finite, *m.dense_grad(x, w, g, biases=b, activation=act, preact=z))
+    _check_grad(x, w, g, act, finite, None, None, m.dense_grad(x, w, g, biases=b, activation=act, preact=z, needs=(False, False))[2])
+    z[1, 2] = float("nan")                             # a NaN still comes through, in its row and column
+    dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z)
+    assert bool(torch.isnan(dx[1]).all()) and bool(torch.isnan(dw[:, 2]).all()) and bool(torch.isnan(db[2]))
+    assert int(torch.isnan(dx).any(1).sum()) == 1 and int(torch.isnan(dw).any(0).sum()) == 1 and int(torch.isnan(db).sum()) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_a_preactivation_that_fp16_keeps_as_an_infinity(gpu, act):
+    """z of +-10^5 is finite in the forward pass's fp32 and +-infinity in the fp16 that the backward pass gets."""
+    m = _mod()
+    dt = torch.float16
+    x, w, g = torch.ones(4, 8, dtype=dt, device=gpu), _rand(gpu, (8, 16), dt, 1), _rand(gpu, (4, 16), dt, 2)
+    w[:, 3], w[:, 5] = -12500.0, 2.0                   # -99968 (12500 is no fp16 number, 12496 is), 16
+    x[2] = 1.0 / 8
+    out, z = m.dense(x, w, activation=act, return_preact=True)
+    assert float(z[0, 3]) == -float("inf") and float(z[2, 3]) == float(w[0, 3])
+    assert bool((out[:, 3] == 0).all()) and bool(torch.isfinite(out).all())
+    dx, dw, db = m.dense_grad(x, w, g, biases=torch.empty(16, device=gpu), activation=act, preact=z)
+    _check_grad(x, w, g, act, z.clamp(-60, 60), dx, dw, db)
+    assert bool((dw[:, 3] == 0).all()) and float(db[3]) == 0
