@@ -12,6 +12,7 @@ fp32 in, fp32 arithmetic; bf16 / fp16 in, fp32 sums, each output rounded once.
 """
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -43,7 +44,7 @@ def _beside(t, name, inputs, *dtypes):
 def _rows(t, cols):
     """[..., cols] as (tensor, address, elements between rows) with the columns contiguous; a view where the strides allow
     it, a copy otherwise."""
-    m = t if t.dim() == 2 else t.reshape(-1, cols)
+    m = t if t.dim() == 2 else t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
     rows = m.shape[0]
     ld, step = m.stride()
     if (step != 1 and cols > 1) or ((ld < cols or ld >= _FAR) and rows > 1):

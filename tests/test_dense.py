@@ -642,3 +642,28 @@ def test_a_preactivation_that_fp16_keeps_as_an_infinity(gpu, act):
     dx, dw, db = m.dense_grad(x, w, g, biases=torch.empty(16, device=gpu), activation=act, preact=z)
     _check_grad(x, w, g, act, z.clamp(-60, 60), dx, dw, db)
     assert bool((dw[:, 3] == 0).all()) and float(db[3]) == 0
+
+
+def test_rows_of_no_columns_keep_their_number():
+    m = _mod()
+    for shape in ((2, 3, 0), (0,), (6, 0), (2, 0, 3, 0)):
+        t, _, ld = m._rows(torch.zeros(shape), 0)
+        assert t.shape == (math.prod(shape[:-1]), 0) and ld >= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_no_input_channels_with_any_leading_dimensions(gpu, dt):
+    m = _mod()
+    w, b = torch.empty(0, 7, dtype=dt, device=gpu), _rand(gpu, (7,), dt, 1)
+    for lead in ((), (3,), (2, 3), (2, 1, 5), (2, 0, 3)):
+        x, r = torch.empty(lead + (0,), dtype=dt, device=gpu), _rand(gpu, lead + (7,), dt, 2)
+        out, z = m.dense(x, w, b, activation="silu", residual=r, return_preact=True)
+        assert out.shape == lead + (7,) and torch.equal(z, b.expand(lead + (7,)))
+        want = _act64(b.double(), "silu") + r.double()
+        _within(out, want, _half(dt) * want.abs() + 40 * U * (1 + want.abs() + r.double().abs()) + _tiny(dt), "out")
+        assert not bool(m.dense(x, w).any())
+        dx, dw, db = m.dense_grad(x, w, r, biases=b)
+        assert dx.shape == x.shape and dw.shape == (0, 7)
+        rd = r.double().view(-1, 7)
+        _within(db, rd.sum(0), _half(dt) * rd.sum(0).abs() + 8 * U * rd.abs().sum(0) + _tiny(dt), "grad_biases")
