@@ -423,6 +423,10 @@ struct Backward {
     bool bias_in_dw;
 };
 constexpr int kWantX = 1, kWantW = 2, kWantB = 4;
+// Those of the wanted gradients that have elements (a plan counts their blocks)
+inline int wanted(bool x, bool w, bool b, long rows, int cin, int cout) {
+    return (x && rows && cin ? kWantX : 0) | (w && cin && cout ? kWantW : 0) | (b && cout ? kWantB : 0);
+}
 // Up to here each small block forms the dZ it reads (a layer of 2^26 products: some 2 us of slopes, spread over the chip;
 // ReLU's cost nothing); beyond, one pass in front does.
 inline double slope_work(int act) { return act <= kRelu ? 1L << 30 : 1L << 26; }
@@ -511,6 +515,9 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
 
 extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes) {
     if (!bytes || !sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu || want < 0 || want > 7) return SA_ERR_INVALID;
+    *bytes = 0;
+    want = wanted(want & kWantX, want & kWantW, want & kWantB, rows, cin, cout);
+    if (!want) return SA_OK;
     Backward b;
     Scratch s{nullptr};
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{nullptr, cin, rows, cin, (flags & 1) != 0},
@@ -524,7 +531,7 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
                                  const void *g, long ldg, const void *z, long ldz, int act, void *dx, void *dw, void *db,
                                  int db_f32, void *ws, unsigned long ws_bytes, void *stream) {
     if (!sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu) return SA_ERR_INVALID;
-    const int want = (dx && rows && cin ? kWantX : 0) | (dw && cin && cout ? kWantW : 0) | (db && cout ? kWantB : 0);
+    const int want = wanted(dx, dw, db, rows, cin, cout);
     if (!want) return SA_OK;
     if (rows && cout && (!g || ldg < cout || (act != kNone && (!z || ldz < cout)))) return SA_ERR_INVALID;
     if ((want & kWantX) && cout && (!w || ldw < cout)) return SA_ERR_INVALID;

@@ -667,3 +667,18 @@ def test_no_input_channels_with_any_leading_dimensions(gpu, dt):
         assert dx.shape == x.shape and dw.shape == (0, 7)
         rd = r.double().view(-1, 7)
         _within(db, rd.sum(0), _half(dt) * rd.sum(0).abs() + 8 * U * rd.abs().sum(0) + _tiny(dt), "grad_biases")
+
+
+def test_scratch_of_empty_layers():
+    """Gradients that an empty layer does not have need no scratch, and asking for it is no error."""
+    lib = pkg("utils._native").lib()
+    n = ctypes.c_ulong()
+    for dtype in range(3):
+        for act in (0, 1, 4):
+            for want in range(8):
+                for rows, cin, cout in ((0, 5, 7), (3, 0, 7), (3, 5, 0), (0, 0, 7), (0, 5, 0), (3, 0, 0), (0, 0, 0), (4000, 0, 4000),
+                                        (0, 4000, 4000), (4000, 4000, 0)):
+                    n.value = 1
+                    assert lib.sa_dense_backward_ws(dtype, rows, cin, cout, act, want, 7, ctypes.byref(n)) == 0
+                    # the column sums of rows that are there are all that takes any
+                    assert n.value == 0 or (want & 4 and rows and cout and not cin)
