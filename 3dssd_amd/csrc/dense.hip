@@ -4,6 +4,8 @@
 #include "dense_common.h"
 #include "dense_products.h"
 
+#include <initializer_list>
+
 using namespace dense;
 
 namespace {
@@ -208,6 +210,15 @@ __global__ __launch_bounds__(1024) void sum_strips_kernel(const float *sums, int
 // ---- host ----------------------------------------------------------------------------------------------------------
 inline long esize(int type) { return type == kF32 ? 4 : 2; }
 inline bool aligned(const void *p, long ld, int type) { return ((uintptr_t)p & 15) == 0 && (ld * esize(type)) % 16 == 0 && ld * esize(type) < 2 * kMaxTileLd; }
+// Whole elements: the buffer loads of the small products would round such an address down
+inline bool whole(int type, std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if ((uintptr_t)p & (esize(type) - 1)) return false;
+    return true;
+}
+inline bool scratch_ok(const void *ws, unsigned long used, unsigned long bytes) {
+    return used == 0 || (ws && ((uintptr_t)ws & 255) == 0 && used <= bytes);
+}
 inline bool sizes_ok(int type, long rows, int cin, int cout) {
     return type >= kF32 && type <= kF16 && rows >= 0 && cin >= 0 && cout >= 0 && cin < kMaxLd && cout < kMaxLd;
 }
@@ -498,12 +509,13 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     if (!sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu) return SA_ERR_INVALID;
     if (rows == 0 || cout == 0) return SA_OK;
     if (!y || (cin && (!x || !w)) || ldx < cin || ldw < cout || (res && ldr < cout)) return SA_ERR_INVALID;
+    if (!whole(dtype, {x, w, res, y, pre}) || !whole(bias_f32 ? kF32 : dtype, {bias})) return SA_ERR_INVALID;
     if (ldx >= kMaxLd || ldw >= kMaxLd) return SA_ERR_UNSUPPORTED;
     Forward f;
     Scratch s{(char *)ws};
     plan_forward(f, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
                  Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)});
-    if (s.used > ws_bytes || (s.used && !ws)) return SA_ERR_INVALID;
+    if (!scratch_ok(ws, s.used, ws_bytes)) return SA_ERR_INVALID;
     Epilogue &e = f.plan.P.e;
     e = Epilogue{y, cout, pre, cout, bias, bias_f32, res, ldr, act};
     const int rc = launch_jobs(dtype, f.jobs, f.njobs, (hipStream_t)stream);
@@ -536,6 +548,7 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     if (rows && cout && (!g || ldg < cout || (act != kNone && (!z || ldz < cout)))) return SA_ERR_INVALID;
     if ((want & kWantX) && cout && (!w || ldw < cout)) return SA_ERR_INVALID;
     if ((want & kWantW) && rows && (!x || ldx < cin)) return SA_ERR_INVALID;
+    if (!whole(dtype, {x, w, g, act == kNone ? nullptr : z, dx, dw}) || !whole(db_f32 ? kF32 : dtype, {db})) return SA_ERR_INVALID;
     if (((want & kWantX) && ldw >= kMaxLd) || ((want & kWantW) && ldx >= kMaxLd) || ldg >= kMaxLd ||
         (act != kNone && ldz >= kMaxLd))
         return SA_ERR_UNSUPPORTED;
@@ -544,7 +557,7 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
                   Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)}, Matrix{g, ldg, rows, cout, aligned(g, ldg, dtype)},
                   Matrix{z, ldz, rows, cout, aligned(z, ldz, dtype)}, act, want);
-    if (s.used > ws_bytes || (s.used && !ws)) return SA_ERR_INVALID;
+    if (!scratch_ok(ws, s.used, ws_bytes)) return SA_ERR_INVALID;
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_jobs(dtype, b.jobs, b.njobs, st);
     if (rc) return rc;

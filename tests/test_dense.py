@@ -682,3 +682,30 @@ def test_scratch_of_empty_layers():
                     assert lib.sa_dense_backward_ws(dtype, rows, cin, cout, act, want, 7, ctypes.byref(n)) == 0
                     # the column sums of rows that are there are all that takes any
                     assert n.value == 0 or (want & 4 and rows and cout and not cin)
+
+
+def test_the_c_entries_refuse_addresses_inside_an_element_and_unaligned_scratch():
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses below: only where nothing could be launched on them")
+    lib = pkg("utils._native").lib()
+    n = ctypes.c_ulong()
+    p = 1 << 20                                        # an address that is never dereferenced: every call below is refused
+    for dtype, off in ((0, 1), (0, 2), (1, 1), (2, 1)):
+        ok = dict(x=p, w=p, bias=p, res=p, y=p, pre=p)
+        for name in ok:
+            a = {**ok, name: p + off}
+            assert lib.sa_dense_forward(dtype, 4, 8, 8, a["x"], 8, a["w"], 8, a["bias"], 0, a["res"], 8, 1, a["y"], a["pre"], None, 0,
+                                        None) == -1, (dtype, off, name)
+        ok = dict(x=p, w=p, g=p, z=p, dx=p, dw=p, db=p)
+        for name in ok:
+            a = {**ok, name: p + off}
+            assert lib.sa_dense_backward(dtype, 4, 8, 8, a["x"], 8, a["w"], 8, a["g"], 8, a["z"], 8, 1, a["dx"], a["dw"], a["db"], 0,
+                                         None, 0, None) == -1, (dtype, off, name)
+    assert lib.sa_dense_forward(1, 4, 8, 8, p, 8, p, 8, p + 2, 1, None, 0, 0, p, None, None, 0, None) == -1      # fp32 bias, fp32 db
+    assert lib.sa_dense_backward(1, 4, 8, 8, p, 8, p, 8, p, 8, None, 0, 0, p, p, p + 2, 1, None, 0, None) == -1
+    assert lib.sa_dense_forward_ws(1, 400, 4096, 8, 3, ctypes.byref(n)) == 0 and n.value > 0
+    for off in (2, 16, 128):
+        assert lib.sa_dense_forward(1, 400, 4096, 8, p, 4096, p, 8, None, 0, None, 0, 0, p, None, p + off, n.value, None) == -1
+    assert lib.sa_dense_backward_ws(1, 4000, 1000, 1000, 0, 7, 7, ctypes.byref(n)) == 0 and n.value > 0
+    for off in (2, 16, 128):
+        assert lib.sa_dense_backward(1, 4000, 1000, 1000, p, 1000, p, 1000, p, 1000, None, 0, 0, p, p, p, 0, p + off, n.value, None) == -1
