@@ -65,7 +65,8 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
 //   as X and W;
 //   or, of a fp32 matrix, three bf16 planes x = h + m + l, each the rounded rest of the one before: 27 bits, so nothing of
 //   x's 24 is lost, and the six products h h, h m, m h, m m, h l, l h of two such operands leave out terms below 2^-24 of
-//   the product -- fp32's own rounding -- at 6 / 16 of the cost of fp32 MFMAs.
+//   the product -- fp32's own rounding -- at 6 / 16 of the cost of fp32 MFMAs.  bf16 ends where fp32's normal range does, with
+//   steps of 2^-133: a x below 2^-110 is held to 2^-134, not to 2^-24 of itself.
 // A thread owns eight columns; a block's threads take 256 columns of eight rows at a time, or of wide matrices 2048 of one
 // (4 KB runs of 16-bit elements).  The row lanes of a block meet in LDS, the strips in
 // sum_strips_kernel, in a fixed order.  Bound by memory: each element is read and written once.
@@ -89,7 +90,8 @@ struct Jobs {
 
 // x finite and too large for bf16 rounds to its largest value (the planes below hold the rest).  An infinity is
 // (+-1, 0, +-infinity): the last plane only meets the other factor's first, which has its sign and is 0 only if the factor
-// is; in the first plane it would meet rests that are 0 or of the other sign, and the sum would be NaN.
+// is; in the first plane it would meet rests that are 0 or of the other sign, and the sum would be NaN.  For that a x of up to
+// 2^-134, which bf16 rounds to 0, has a step (2^-133) in its first plane that the second takes back.
 __device__ __forceinline__ void three_planes(float x, unsigned short (&o)[3]) {
     float r = x;
 #pragma unroll
@@ -99,11 +101,15 @@ __device__ __forceinline__ void three_planes(float x, unsigned short (&o)[3]) {
         o[i] = h;
         r -= __uint_as_float((unsigned)h << 16);
     }
+    const unsigned short sign = x < 0.0f ? 0x8000 : 0;
     if (fabsf(x) == __builtin_inff()) {
-        const unsigned short sign = x < 0.0f ? 0x8000 : 0;
         o[0] = sign | 0x3f80;
         o[1] = 0;
         o[2] = sign | 0x7f80;
+    }
+    if ((o[0] & 0x7fff) == 0 && x != 0.0f) {
+        o[0] = sign | 1;
+        o[1] = (sign ^ 0x8000) | 1;
     }
 }
 

@@ -1,6 +1,7 @@
 // Large fp32 layers on bf16 matrix instructions: D(m,n) = sum_k A(m,k) B(k,n) with A in fp32 (k contiguous) and B as three
 // bf16 planes (dense.hip).  A's values become three planes x = h + m + l on their way, and the six products l h, m m, m h,
-// h l, h m, h h of every pair go into one fp32 sum: 24 bits of each factor, at 6 / 16 of the cost of fp32 matrix instructions.
+// h l, h m, h h of every pair go into one fp32 sum: 24 bits of each factor (of one below 2^-110 those from
+// 2^-134 on), at 6 / 16 of the cost of fp32 matrix instructions.
 //
 // Against the tile kernel run six times over planes of both (dense_tile.hip): A is read once, as 4 bytes instead of six times
 // 2; no pass in front has to write 6 bytes for each of its values; and a fragment serves two or three products while it is in
@@ -51,22 +52,30 @@ struct Splitting {
             x[2 * p + 1] -= __uint_as_float(v & 0xffff0000u);
         }
     }
-    // After the last part: an infinity becomes (+-1, 0, +-infinity), as in dense.hip.  So far it is (largest, infinity, NaN),
-    // and its last rest, like a NaN's and no other's, is NaN.
-    __device__ __forceinline__ void infinities() {
+    // After the last part: an infinity becomes (+-1, 0, +-infinity), and a value of up to 2^-134 (+-2^-133, -+2^-133, 0), as in
+    // dense.hip.  So far the former is (largest, infinity, NaN), and its last rest is NaN, like a NaN's; the latter is three
+    // zeros, and its last rest, itself, is below the normal range, like those of values below 2^-109.
+    __device__ __forceinline__ void far_ends() {
         bool some = false;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) some |= __builtin_isunordered(x[2 * p], x[2 * p + 1]);
+        for (int p = 0; p < 8; ++p) some |= __builtin_amdgcn_classf(x[p], 0x93);           // NaN, subnormal
         if (__builtin_expect(__ballot(some) != 0, 0)) {
 #pragma unroll
             for (int p = 0; p < 4; ++p)
 #pragma unroll
                 for (int at = 0; at < 32; at += 16) {
-                    const unsigned m = plane[1][p] >> at & 0xffff, sign = m & 0x8000, mask = 0xffffu << at;
-                    if ((m & 0x7fff) != 0x7f80) continue;
-                    plane[0][p] = (plane[0][p] & ~mask) | (sign | 0x3f80) << at;
-                    plane[1][p] &= ~mask;
-                    plane[2][p] = (plane[2][p] & ~mask) | (sign | 0x7f80) << at;
+                    const unsigned m = plane[1][p] >> at & 0xffff, mask = 0xffffu << at;
+                    const float rest = x[2 * p + at / 16];
+                    if ((m & 0x7fff) == 0x7f80) {
+                        const unsigned sign = m & 0x8000;
+                        plane[0][p] = (plane[0][p] & ~mask) | (sign | 0x3f80) << at;
+                        plane[1][p] &= ~mask;
+                        plane[2][p] = (plane[2][p] & ~mask) | (sign | 0x7f80) << at;
+                    } else if ((plane[0][p] >> at & 0x7fff) == 0 && rest != 0.0f) {
+                        const unsigned sign = __float_as_uint(rest) >> 16 & 0x8000;
+                        plane[0][p] = (plane[0][p] & ~mask) | (sign | 1) << at;
+                        plane[1][p] = (plane[1][p] & ~mask) | ((sign ^ 0x8000) | 1) << at;
+                    }
                 }
         }
     }
@@ -145,7 +154,7 @@ __global__ __launch_bounds__(W * 64, 2) void split_kernel(Product P) {
         }
     };
     auto keep_a = [&](int g, unsigned to) __attribute__((always_inline)) {
-        s[g].infinities();
+        s[g].far_ends();
 #pragma unroll
         for (int p = 0; p < 3; ++p) *(lds_w4)(uintptr_t)(to + p * kPlane + g * (kPlane / 2) + put) = s[g].plane[p];
     };

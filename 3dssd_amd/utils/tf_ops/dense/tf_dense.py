@@ -8,7 +8,9 @@ activation and residual in the product's epilogue, and with a backward pass.  Li
 
     z = inputs @ weights + biases,   out = activation(z) + residual
 
-fp32 in, fp32 arithmetic; bf16 / fp16 in, fp32 sums, each output rounded once.
+fp32 in, fp32 arithmetic; bf16 / fp16 in, fp32 sums, each output rounded once.  Large fp32 layers take their factors apart into
+bf16 planes: a factor is held to 2^-24 of itself or to 2^-134, whichever is larger (below 2^-110 that is fewer than 24 bits:
+scale such operands by a power of two), and a sum within a hundredth of the largest fp32 number may become infinite.
 """
 import ctypes
 import functools

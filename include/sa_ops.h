@@ -256,9 +256,10 @@ int sa_dense(long rows, int K, int N, const float *x, const void *wpack, const f
  * (ldw), res [rows,cout] (ldr; nullable), y and pre [rows,cout] (dense; pre = x W + bias, nullable); bias [cout] (nullable)
  * is fp32 where bias_f32 is set, else of that type.  act: 0 none, 1 ReLU, 2 GELU (normal integral), 3 GELU (tanh form),
  * 4 SiLU.  Any alignments of whole elements (-1 otherwise); cin and cout below 2^24 (-1 otherwise), and ldx and ldw (-3
- * otherwise); sums in fp32, one rounding per output, no atomics: the same call gives the same bits.  ws:
- * sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has a 16-byte aligned base and row length, and rows less than 4 MB
- * apart), 256-byte aligned (-1 otherwise), used until the call's work on the stream is done. */
+ * otherwise); sums in fp32, one rounding per output, no atomics: the same call gives the same bits.  Large fp32 layers hold
+ * a factor to 2^-24 of itself or to 2^-134, whichever is larger, and a sum within 1/100 of the largest number may overflow.
+ * ws: sa_dense_forward_ws bytes (flags: bit 0 / 1 = x / W has a 16-byte aligned base and row length, and rows less than
+ * 4 MB apart), 256-byte aligned (-1 otherwise), used until the call's work on the stream is done. */
 int sa_dense_forward_ws(int dtype, long rows, int cin, int cout, int flags, unsigned long *bytes);
 int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
                      const void *bias, int bias_f32, const void *res, long ldr, int act, void *y, void *pre, void *ws,

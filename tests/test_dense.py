@@ -709,3 +709,199 @@ def test_the_c_entries_refuse_addresses_inside_an_element_and_unaligned_scratch(
     assert lib.sa_dense_backward_ws(1, 4000, 1000, 1000, 0, 7, 7, ctypes.byref(n)) == 0 and n.value > 0
     for off in (2, 16, 128):
         assert lib.sa_dense_backward(1, 4000, 1000, 1000, p, 1000, p, 1000, p, 1000, None, 0, 0, p, p, p, 0, p + off, n.value, None) == -1
+
+
+# ------------------------------------------------------------------------------- large fp32 products: bits and ranges of a factor
+def _planes(v):
+    """v = h + m + l + what 27 bits do not hold, each plane bf16 (CPU)."""
+    out = []
+    for _ in range(3):
+        p = v.to(torch.bfloat16).float()
+        out.append(p)
+        v = v - p
+    return out
+
+
+PLANE_PRODUCTS = [(0, 0), (0, 1), (1, 0), (1, 1), (0, 2), (2, 0)]
+# Of |x w|.  Left out are m l and l m, at most 2^-27 each (m is within 2^-9 of the factor, l within 2^-18), and what is behind
+# either factor's third plane, 2^-27 each: 2^-25 or U / 2.  An addition to a sum of the product's size is off by a step, 2 U, at
+# the most, one below 2^-8 of that size by nothing that counts.  There are up to four of those: the split kernel's last block adds
+# h h third, and m m, h m and h l behind it; elsewhere h h comes last.  8.5 U, against 2^-18 = 64 U and more of a whole l h or m m.
+SINGLE_TERM = 9 * U
+
+
+def _factors(shape, seed, device="cpu"):
+    """Random 24-bit mantissas, signs, and exponents from -20 to 20; a few with planes as large as they get."""
+    g = torch.Generator().manual_seed(seed)
+    v = (1 + torch.rand(shape, generator=g, dtype=torch.float64)).float() * torch.exp2(torch.randint(-20, 21, shape, generator=g).float())
+    v = torch.where(torch.rand(shape, generator=g) < 0.5, -v, v)
+    v.view(-1)[::7] = 1 + 2.0 ** -8 * (1 - 2.0 ** -7) + 2.0 ** -17
+    return v.to(device)
+
+
+def test_a_missing_plane_product_shows_in_a_single_term():
+    """The bound below sees each of the six products: without any one of them a CPU emulation is outside."""
+    x, w = _factors((4000,), 1), _factors((4000,), 2)
+    px, pw = _planes(x), _planes(w)
+    want = x.double() * w.double()
+    for missing in [None] + PLANE_PRODUCTS:
+        got = sum(px[a].double() * pw[b].double() for a, b in PLANE_PRODUCTS if (a, b) != missing).float().double()
+        inside = bool(((got - want).abs() <= SINGLE_TERM * want.abs()).all())
+        assert inside == (missing is None), missing
+
+
+SINGLE_FORWARD = {"split": (2048, 512, 8192), "tiles": (2048, 512, 2048)}
+SINGLE_WEIGHTS = {"split": (300, 4096, 4096), "tiles": (300, 8192, 1024), "pieces": (4096, 1024, 1024)}
+
+
+def test_both_kernels_of_large_fp32_products_are_met():
+    """By their scratch: the tiles have planes of both factors there, the split kernel of the second only."""
+    lib = pkg("utils._native").lib()
+    n = ctypes.c_ulong()
+    up = lambda v, m: (v + m - 1) // m * m  # noqa: E731
+    planes = lambda rows, cols: up(6 * rows * up(cols, 64), 256)  # noqa: E731
+    for kernel, (rows, cin, cout) in SINGLE_FORWARD.items():
+        assert lib.sa_dense_forward_ws(0, rows, cin, cout, 3, ctypes.byref(n)) == 0
+        assert n.value == planes(cin, cout) + (planes(rows, cin) if kernel == "tiles" else 0)
+    for kernel, (rows, cin, cout) in SINGLE_WEIGHTS.items():
+        assert lib.sa_dense_backward_ws(0, rows, cin, cout, 0, 2, 7, ctypes.byref(n)) == 0
+        least = planes(rows, cout) + (planes(rows, cin) if kernel == "tiles" else 0)
+        assert n.value > least if kernel == "pieces" else n.value == least
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", sorted(SINGLE_FORWARD))
+def test_every_bit_of_a_single_term(gpu, kernel):
+    """One nonzero factor per sum: no other term hides the bits of its product."""
+    m = _mod()
+    rows, cin, cout = SINGLE_FORWARD[kernel]
+    x, w = torch.zeros(rows, cin, device=gpu), _factors((cin, cout), 1, gpu)
+    at = torch.arange(rows, device=gpu) * 37 % cin
+    v = _factors((rows,), 2, gpu)
+    x[torch.arange(rows, device=gpu), at] = v
+    want = v.double()[:, None] * w.double()[at]
+    _within(m.dense(x, w), want, SINGLE_TERM * want.abs(), "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", sorted(SINGLE_WEIGHTS.values()))
+def test_every_bit_of_a_single_term_of_the_gradient(gpu, size):
+    m = _mod()
+    rows, cin, cout = size
+    r = torch.arange(rows, device=gpu)
+    # grad_inputs: one nonzero grad_out per row
+    g, w, x = torch.zeros(rows, cout, device=gpu), _factors((cin, cout), 1, gpu), _factors((rows, cin), 2, gpu)
+    at, v = r * 37 % cout, _factors((rows,), 3, gpu)
+    g[r, at] = v
+    want = v.double()[:, None] * w.double().t().contiguous()[at]
+    _within(m.dense_grad(x, w, g, needs=(True, False))[0], want, SINGLE_TERM * want.abs(), "grad_inputs")
+    # grad_weights: one nonzero input per channel
+    g, x = _factors((rows, cout), 4, gpu), torch.zeros(rows, cin, device=gpu)
+    c = torch.arange(cin, device=gpu)
+    at, v = (c * 41 + 5) % rows, _factors((cin,), 5, gpu)
+    x[at, c] = v
+    want = v.double()[:, None] * g.double()[at]
+    for needs in ((False, True), (True, True)):
+        _within(m.dense_grad(x, w, g, needs=needs)[1], want, SINGLE_TERM * want.abs(), "grad_weights")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_negative_tails_are_relatively_right(gpu, act):
+    """fp32, one channel of weight 1, so z is the input.  The value in the tail is an exponential: a rounding of its exponent by u
+    relative shows times the exponent.  GELU: exponent z^2 / 2, two roundings and a constant: 1.5 z^2 u; polynomial, reciprocals
+    (two steps each), exponential and products: 24 u.  SiLU: 2 |z| u and 12 u.  Tanh form: exponent 2 sqrt(2/pi) (z + 0.044715 z^3)
+    with seven roundings and two constants: 10 u of it, and 12 u.  The slopes are sums of two such terms,
+    the second with s (1 - s): twice the error of s."""
+    m = _mod()
+    low = {"gelu": -12.8, "gelu_tanh": -9.8, "silu": -85.0}[act]
+    x = torch.linspace(low, 0, 20001, device=gpu)[:, None]
+    one = torch.ones(1, 1, device=gpu)
+    z = x.double()
+    e = {"gelu": 24 + 1.5 * z * z, "silu": 12 + 2 * z.abs(), "gelu_tanh": 12 + 10 * 1.5957691216 * (z.abs() + 0.044715 * z.abs() ** 3)}[act] * U
+    # (tanh and ndtr of torch lose the tails: the formulas without a difference)
+    if act == "gelu":
+        p = 0.5 * torch.erfc(-z / math.sqrt(2))
+        second = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        u, du = (z, 1.0) if act == "silu" else (2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3),
+                                                2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z))
+        p = torch.exp(u) / (1 + torch.exp(u))
+        second = z * p / (1 + torch.exp(u)) * du
+    out, pre = m.dense(x, one, activation=act, return_preact=True)
+    assert torch.equal(pre, x)
+    _within(out, z * p, e * (z * p).abs() + 1e-45, "out")
+    slope = m.dense_grad(x, one, torch.ones_like(x), activation=act, preact=x, needs=(True, False))[0]
+    _within(slope, p + second, (2 * e + 8 * U) * (p + second.abs()), "slope")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(70, 129, 65), (2048, 512, 2048), (2048, 512, 8192)])
+def test_tiny_fp32_factors(gpu, size):
+    """Large products hold a fp32 factor to 2^-24 of itself or to 2^-134, half of the smallest step of its planes, whichever is
+    larger; small ones to all of its bits.  And an infinity times anything but 0 and NaN is an infinity.
+    (A factor below 2^-126 enters the matrix instructions unnormalised, as 2^-126 times a fraction: a sum with it keeps 24 bits from
+    2^-126 times the other factor down, so that each of the six products may be off by 2^-149 times the other factor.)"""
+    m = _mod()
+    held = 2.0 ** -134 + 6 * 2.0 ** -149
+    rows, cin, cout = size
+    r = torch.arange(rows, device=gpu)
+    at = r * 37 % cin
+    w = _factors((cin, cout), 1, gpu) * 2.0 ** 70      # 2^50 to 2^91
+    for e in (-100, -108, -114, -120, -126):
+        v = _factors((rows,), 2, gpu).sign() * (1 + torch.rand(rows, generator=torch.Generator().manual_seed(3))).to(gpu) * 2.0 ** e
+        x = torch.zeros(rows, cin, device=gpu)
+        x[r, at] = v
+        want = v.double()[:, None] * w.double()[at]
+        step = held * w.double().abs()[at] * (rows > 100)
+        _within(m.dense(x, w), want, SINGLE_TERM * want.abs() + step, "out")
+        # the same with the factors' parts exchanged: W tiny, X large
+        tiny = torch.ldexp(_factors((cin, cout), 4, gpu), torch.tensor(e - 20, device=gpu))
+        x[r, at] = _factors((rows,), 5, gpu) * 2.0 ** 100
+        want = x[r, at].double()[:, None] * tiny.double()[at]
+        step = held * x[r, at].double().abs()[:, None] * (rows > 100)
+        _within(m.dense(x, tiny), want, SINGLE_TERM * want.abs() + step, "out, tiny weights")
+    # infinities
+    inf = float("inf")
+    tiny = torch.tensor([1e-30, 2.0 ** -126, 2.0 ** -133, 2.0 ** -134, 1.5 * 2.0 ** -134, 2.0 ** -135, 2.0 ** -149, 0.0, 1e-40], dtype=torch.float64)
+    tiny = torch.cat([tiny, -tiny]).float().to(gpu)
+    assert int((tiny != 0).sum()) == 16
+    ones = torch.ones(rows, device=gpu)
+    ones[1::2] = -1
+
+    def signs(got, want, what):
+        for a, b in ((torch.isnan(got), torch.isnan(want)), (got == inf, want == inf), (got == -inf, want == -inf)):
+            assert torch.equal(a, b), what
+
+    x, w = torch.zeros(rows, cin, device=gpu), tiny.repeat(cin * cout // 18 + 1)[:cin * cout].view(cin, cout).contiguous()
+    x[r, at] = ones * inf
+    signs(m.dense(x, w), (ones * inf)[:, None] * w[at], "infinite inputs, tiny weights")
+    g = torch.zeros(rows, cout, device=gpu)
+    to = r * 37 % cout
+    g[r, to] = ones * inf
+    signs(m.dense_grad(x, w, g, needs=(True, False))[0], (ones * inf)[:, None] * w.t()[to], "infinite grad_out, tiny weights")
+    x[r, at] = tiny.repeat(rows // 18 + 1)[:rows]
+    full = torch.where(x == 0, 2.0 ** -140, x)         # tiny factors all along a row, of one sign
+    full = full.abs() * ones[:, None]
+    w = torch.full((cin, cout), inf, device=gpu)
+    w[:, 1::2] = -inf
+    signs(m.dense(full, w), (ones * inf)[:, None] * w[:1], "tiny inputs, infinite weights")
+    c = torch.arange(cin, device=gpu)
+    x, g = torch.zeros(rows, cin, device=gpu), torch.full((rows, cout), 2.0 ** -141, device=gpu)
+    x[(c * 41 + 5) % rows, c] = inf
+    signs(m.dense_grad(x, w, g, needs=(False, True))[1], torch.full((cin, cout), inf, device=gpu), "infinite inputs, tiny grad_out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(70, 129, 65), (2048, 512, 2048), (2048, 512, 8192)])
+def test_fp32_products_near_the_largest_number(gpu, size):
+    # the first planes may be larger than their factors, by 2^-8 each: a product up to the largest number / 1.008 does not overflow
+    m = _mod()
+    rows, cin, cout = size
+    g = torch.Generator(device=gpu).manual_seed(1)
+    r = torch.arange(rows, device=gpu)
+    at = r * 37 % cin
+    x, w = torch.zeros(rows, cin, device=gpu), 1 - 0.1 * torch.rand(cin, cout, generator=g, device=gpu)
+    x[r, at] = (torch.finfo(torch.float32).max / 1.008) * (1 - 0.1 * torch.rand(rows, generator=g, device=gpu))
+    want = x[r, at].double()[:, None] * w.double()[at]
+    _within(m.dense(x, w), want, SINGLE_TERM * want.abs(), "out")
