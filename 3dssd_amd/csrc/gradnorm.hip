@@ -120,16 +120,24 @@ __global__ __launch_bounds__(256) void norm_kernel(const double *partial, int co
     if (threadIdx.x == 0) *norm = v;
 }
 
+// What a gradient is multiplied by: `by`, after a power of two where the factor is below 2^-100.  There one fp32 number would have
+// lost bits, or been 0, while the products are ordinary numbers (1e36 clipped to 1e-9).
+struct Factor {
+    float first, by;
+};
+template <class T>
+__device__ __forceinline__ T scaled(T g, Factor f) { return from_f32<T>(to_f32<T>(g) * f.first * f.by); }
+
 template <class T, bool STREAM>
-__device__ __forceinline__ void scale_chunk(const T *p, T *o, long n, float f) {
+__device__ __forceinline__ void scale_chunk(const T *p, T *o, long n, Factor f) {
     constexpr int V = 16 / sizeof(T);
     struct alignas(16) Pack { T x[V]; };
     if ((((uintptr_t)p ^ (uintptr_t)o) & 15) != 0) {                     // source and result differ in alignment
-        for (long i = threadIdx.x; i < n; i += 256) o[i] = from_f32<T>(to_f32<T>(p[i]) * f);
+        for (long i = threadIdx.x; i < n; i += 256) o[i] = scaled<T>(p[i], f);
         return;
     }
     const int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
-    if ((int)threadIdx.x < head && threadIdx.x < n) o[threadIdx.x] = from_f32<T>(to_f32<T>(p[threadIdx.x]) * f);
+    if ((int)threadIdx.x < head && threadIdx.x < n) o[threadIdx.x] = scaled<T>(p[threadIdx.x], f);
     if (n <= head) return;
     const Pack *q = (const Pack *)(p + head);
     Pack *w = (Pack *)(o + head);
@@ -144,7 +152,7 @@ __device__ __forceinline__ void scale_chunk(const T *p, T *o, long n, float f) {
 #pragma unroll
         for (int i = 0; i < kChunk / 16 / 256; ++i) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i].x[j] = from_f32<T>(to_f32<T>(v[i].x[j]) * f);
+            for (int j = 0; j < V; ++j) v[i].x[j] = scaled<T>(v[i].x[j], f);
             if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(u4, v[i]), (u4 *)w + threadIdx.x + 256 * i);
             else w[threadIdx.x + 256 * i] = v[i];
         }
@@ -153,11 +161,11 @@ __device__ __forceinline__ void scale_chunk(const T *p, T *o, long n, float f) {
     for (int i = threadIdx.x; i < packs; i += 256) {
         Pack v = q[i];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v.x[j] = from_f32<T>(to_f32<T>(v.x[j]) * f);
+        for (int j = 0; j < V; ++j) v.x[j] = scaled<T>(v.x[j], f);
         w[i] = v;
     }
     const int done = head + packs * V;
-    if (done + (int)threadIdx.x < n) o[done + threadIdx.x] = from_f32<T>(to_f32<T>(p[done + threadIdx.x]) * f);
+    if (done + (int)threadIdx.x < n) o[done + threadIdx.x] = scaled<T>(p[done + threadIdx.x], f);
 }
 
 // partial null: the norm is read from `given`.  norm_out may be null.
@@ -168,12 +176,19 @@ __global__ __launch_bounds__(256) void scale_kernel(List L, const double *partia
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     // a norm that is NaN, infinite or (given) negative scales by NaN
     const bool ok = norm >= 0.0f && norm <= 3.402823466e38f;
-    const float f = !ok ? __builtin_nanf("") : norm > clip ? (float)((double)clip / (double)norm) : 1.0f;
+    double exact = !ok ? __builtin_nan("") : norm > clip ? (double)clip / (double)norm : 1.0;
+    Factor f{1.0f, 0.0f};
+    if (exact < 0x1p-100) {                            // down to 2^-277: half of the exponent first, as far as fp32 goes
+        const int half = ilogb(exact) / 2;
+        f.first = ldexpf(1.0f, half > -126 ? half : -126);
+        exact /= f.first;
+    }
+    f.by = (float)exact;
     const int total = L.first[L.count];
     int t = L.count - 1;
     for (int c = total - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         while (c < L.first[t]) --t;
-        if (f == 1.0f && L.out[t] == L.p[t]) continue;
+        if (f.by == 1.0f && L.out[t] == L.p[t]) continue;
         const int type = L.type[t], per = per_chunk(type);
         const long at = (long)(c - L.first[t]) * per, left = L.n[t] - at, n = left < per ? left : per;
         if (type == kF32) scale_chunk<float, STREAM>((const float *)L.p[t] + at, (float *)L.out[t] + at, n, f);

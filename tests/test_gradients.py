@@ -243,3 +243,20 @@ def test_a_tensor_of_more_than_32_bits_of_elements(gpu):
     # one division of 64 bits, two roundings to fp32 and one to bf16
     assert all(abs(float(v) - want / 66.0 ** 0.5) <= 2.0 ** -7.9 * want / 66.0 ** 0.5 for v, want in ((t[0], 3.0), (t[-1], 4.0)))
     assert int((t != 0).sum()) == 5
+
+
+@pytest.mark.gpu
+def test_factors_below_the_normal_range(gpu):
+    """clip / norm may be as small as 1e-46 / 1e38 while the clipped values are ordinary numbers."""
+    m = _mod()
+    for v, clip in ((1e36, 1e-3), (1e36, 1e-9), (1e35, 1e-20), (3e36, 3.0), (3e33, 1e-5), (3e37, 5.0)):
+        ts = [torch.full((40,), v, device=gpu), torch.full((3,), -v / 3, device=gpu).to(BF16), _rand(gpu, (77,), F32, 1, v / 10),
+              _rand(gpu, (9,), F16, 2)]
+        into = [torch.full((t.numel() + 1,), 9.0, dtype=t.dtype, device=gpu)[1:] for t in ts]     # aligned unlike the gradients
+        mine = [t.clone() for t in ts]
+        for kw in ({}, {"out": into}, {"out": mine}):
+            src = mine if "out" in kw and kw["out"] is mine else ts
+            got, norm = m.clip_by_global_norm(src, clip, **kw)
+            _check(ts, clip, got, norm)
+    big = [torch.full((20000,), 1e35, device=gpu)]     # whole chunks too
+    _check(big, 1e-8, *m.clip_by_global_norm(big, 1e-8))
