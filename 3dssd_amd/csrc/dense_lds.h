@@ -24,9 +24,9 @@ template <> __device__ __forceinline__ f4 mfma<f16_t>(s8 a, s8 b, f4 c) {
 // 16 bytes per lane from buffer r + off to LDS `to` + 16 lane.  Written as assembly because the compiler, which knows the
 // builtin's loads by the LDS they write, waits for all of them in front of the next read of any LDS -- the other buffer's
 // included -- and the loads would never fly under the products.  Nothing comes back in registers; the kernel waits for
-// vmcnt itself, in front of the barrier that publishes the buffer.  (Nothing else in the kernel uses m0.)
+// vmcnt itself, in front of the barrier that publishes the buffer.
 __device__ __forceinline__ void lds_load(u4 r, unsigned off, unsigned to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(to) : "memory", "m0");
 }
 
 __device__ __forceinline__ u4 buffer(const char *p, unsigned bytes) {
