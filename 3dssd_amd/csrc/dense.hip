@@ -61,8 +61,8 @@ __global__ __launch_bounds__(256) void join_kernel(Product P) {
 //   dZ = G act'(Z), where there is a Z (ReLU selects: what a closed unit receives, infinities among it, does not come
 //   through), and the column sums of dZ, taken before any rounding;
 //   a copy in the layer's type with 16-byte aligned rows, zeros behind the last column up to a multiple of 8 -- for the
-//   tile kernel, whose loads are 16 bytes wide.  dZ is rounded to the layer's type here: it is an operand of the same MFMAs
-//   as X and W;
+//   tile kernel, whose loads are 16 bytes wide.  A 16-bit layer's dZ goes in two planes (dense_common.h), or, where the caller
+//   asks for it, rounded to the layer's type: it is an operand of the same MFMAs as X and W;
 //   or, of a fp32 matrix, three bf16 planes x = h + m + l, each the rounded rest of the one before: 27 bits, so nothing of
 //   x's 24 is lost, and the six products h h, h m, m h, m m, h l, l h of two such operands leave out terms below 2^-24 of
 //   the product -- fp32's own rounding -- at 6 / 16 of the cost of fp32 MFMAs.  bf16 ends where fp32's normal range does, with
@@ -78,7 +78,7 @@ struct Job {
     int cols;
     void *dst;            // [rows][ldd], or null: sums only
     long ldd;             // copied_ld(cols)
-    long plane;           // elements between planes; 0: one copy in the layer's type
+    long plane;           // elements between planes (fp32: three, else two); 0: one copy in the layer's type
     float *sums;          // [strips][cols], or null
     long strip;           // rows of a block
     int wide;             // 2048 columns of a row at a time
@@ -162,6 +162,14 @@ __global__ __launch_bounds__(256) void prepare_kernel(Jobs J) {
                         }
 #pragma unroll
                         for (int p = 0; p < 3; ++p) store_pack<bf16_t, 8>((bf16_t *)S.dst + p * S.plane + at, o[p]);
+                    } else if (sizeof(T) == 2 && S.plane) {
+                        if constexpr (sizeof(T) == 2) {
+                            Eight<T> o[2];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) split_slope<T>(d[i], o[0].x[i], o[1].x[i]);
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) store_pack<T, 8>((T *)S.dst + p * S.plane + at, o[p]);
+                        }
                     } else {
                         Eight<T> o;
 #pragma unroll
@@ -314,11 +322,12 @@ struct Plan {
 };
 enum Kind { kSmall, kTiles, kSplit };
 // Chooses shape and pieces; returns the time to expect (ns; tiles only).
-double plan(Plan &L, int type, Kind kind, bool ta, bool tb, long M, long N, long K) {
+double plan(Plan &L, int type, Kind kind, bool ta, bool tb, long M, long N, long K, bool two = false) {
     Product &P = L.P;
     L.ta = ta; L.tb = tb;
     P.M = M; P.N = N; P.K = K;
-    P.passes = type == kF32 && kind == kTiles ? 6 : 1;
+    P.two = two;
+    P.passes = kind != kTiles ? 1 : type == kF32 ? 6 : two ? 2 : 1;
     auto count = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
     const long unit = kind == kTiles ? 64 : 32, steps = (K + unit - 1) / unit * P.passes;
     long pieces = 1;
@@ -444,16 +453,28 @@ constexpr int kWantX = 1, kWantW = 2, kWantB = 4;
 inline int wanted(bool x, bool w, bool b, long rows, int cin, int cout) {
     return (x && rows && cin ? kWantX : 0) | (w && cin && cout ? kWantW : 0) | (b && cout ? kWantB : 0);
 }
-// Up to here each small block forms the dZ it reads (a layer of 2^26 products: some 2 us of slopes, spread over the chip;
-// ReLU's cost nothing); beyond, one pass in front does.
-inline double slope_work(int act) { return act <= kRelu ? 1L << 30 : 1L << 26; }
+// Whether each small block forms the dZ it reads, or a pass in front does: every block forms it anew, but the pass costs a launch and
+// a round trip to memory.  Formed / with the pass, us: ReLU (a select) fp32 2048 x 128 x 256 12.8 / 19.4, 128 x 4096 x 1024 63 / 59,
+// 16384 x 32 x 2048 82 / 142; GELU fp32 2048 x 128 x 256 16.3 / 19.7, 2048 x 256 x 256 26.4 / 25.9, 2048 x 512 x 256 40 / 35; rounded
+// bf16 512 x 128 x 256 10.1 / 12.0, 2048 x 128 x 256 23 / 17, 64 x 2048 x 2048 48 / 28.  In two planes the slopes of a wave's steps of k
+// weigh more: bf16 GELU 512 x 128 x 256 10.5 / 12.9, 768 x 384 x 384 14.5 / 17.1, 640^3 30 / 26, 4 x 1024 x 4096 50 / 25,
+// 4096 x 16 x 256 47 / 27.
+bool slopes_formed(int type, long rows, int cin, int cout, int act, bool two) {
+    const double products = (double)rows * cin * cout;
+    if (!two) return products <= (act <= kRelu ? 1L << 30 : 1L << 26);
+    if (products > 1L << 27 || products == 0) return products == 0;
+    Plan x{}, w{};
+    plan(x, type, kSmall, false, false, rows, cin, cout);
+    plan(w, type, kSmall, true, true, cin, cout, rows);
+    return x.P.kchunk <= 768 && w.P.kchunk <= 768;
+}
 
 void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int cout, Matrix x, Matrix w, Matrix g, Matrix z,
-                   int act, int want) {
+                   int act, bool two, int want) {
     b = Backward{};
     b.tiles = wants_tiles(type, rows, cin, cout, !tile_operand(type, x) || !tile_operand(type, w), true);
     const bool products = want & (kWantX | kWantW);
-    const bool formed = !b.tiles && (double)rows * cin * cout <= slope_work(act);
+    const bool formed = !b.tiles && slopes_formed(type, rows, cin, cout, act, two);
     Job j{};
     j.g = g.p; j.ldg = g.ld; j.z = act == kNone ? nullptr : z.p; j.ldz = z.ld; j.act = act;
     j.rows = rows; j.cols = cout; j.ldd = copied_ld(cout);
@@ -461,9 +482,9 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     Matrix d = g;
     const bool copy = products && (b.tiles ? act != kNone || !tile_operand(type, g) : act != kNone && !formed);
     if (copy) {
-        const bool planes = b.tiles && type == kF32;
-        j.dst = ws.take((unsigned long)rows * j.ldd * (planes ? 6 : esize(type)));
-        j.plane = planes ? rows * j.ldd : 0;
+        const int planes = type != kF32 ? 1 + two : b.tiles ? 3 : 1;
+        j.dst = ws.take((unsigned long)rows * j.ldd * (planes > 1 ? 2 * planes : esize(type)));
+        j.plane = planes > 1 ? rows * j.ldd : 0;
         d = Matrix{j.dst, j.ldd, rows, cout, true, j.plane};
     }
     b.bias_in_dw = (want & kWantB) && (want & kWantW) && !b.tiles && !copy;
@@ -474,19 +495,23 @@ void plan_backward(Backward &b, Scratch &ws, int type, long rows, int cin, int c
     if (rows && cout && (copy || j.sums)) add_job(b.jobs, b.njobs, j);
     const Kind kind = b.tiles ? kTiles : kSmall;
     if (want & kWantW) {
-        const double time = plan(b.dw, type, kind, true, true, cin, cout, rows);
+        const double time = plan(b.dw, type, kind, true, true, cin, cout, rows, two);
         if (b.tiles && type == kF32 && prefer_split(b.dw, time, x, true)) copy_for_split(b.jobs, b.njobs, ws, x);
         else if (b.tiles && !tile_operand(type, x)) copy_for_tiles(b.jobs, b.njobs, ws, type, x);
     }
     if (b.tiles && (want & kWantX) && !tile_operand(type, w)) copy_for_tiles(b.jobs, b.njobs, ws, type, w);
     if (want & kWantX) {
-        plan(b.dx, type, kind, false, false, rows, cin, cout);
+        plan(b.dx, type, kind, false, false, rows, cin, cout, two);
         place(b.dx, ws, d, w);
     }
     if (want & kWantW) place(b.dw, ws, x, d);
     if (act != kNone && !copy) {
         for (Product *P : {&b.dx.P, &b.dw.P}) {
             P->z = z.p; P->ldz = z.ld; P->vec_z = z.vec; P->zact = act;
+        }
+    } else if (two && !b.tiles) {
+        for (Product *P : {&b.dx.P, &b.dw.P}) {
+            P->z = (const char *)d.p + d.plane * 2; P->ldz = d.ld; P->vec_z = 1; P->zact = kPlanes;
         }
     }
     if (b.bias_in_dw && b.dw.P.splits > 1) {
@@ -531,8 +556,17 @@ extern "C" int sa_dense_forward(int dtype, long rows, int cin, int cout, const v
     return rs ? rs : launch_join(dtype, f.plan.P, (hipStream_t)stream);
 }
 
-extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes) {
-    if (!bytes || !sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu || want < 0 || want > 7) return SA_ERR_INVALID;
+// An activation, with kRoundSlopes added or without, and whether dZ goes in two planes
+inline bool take_act(int type, int given, int &act, bool &two) {
+    act = given & ~kRoundSlopes;
+    two = type != kF32 && act > kRelu && !(given & kRoundSlopes);
+    return act >= kNone && act <= kSilu;
+}
+
+extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int activation, int want, int flags, unsigned long *bytes) {
+    int act;
+    bool two;
+    if (!bytes || !sizes_ok(dtype, rows, cin, cout) || !take_act(dtype, activation, act, two) || want < 0 || want > 7) return SA_ERR_INVALID;
     *bytes = 0;
     want = wanted(want & kWantX, want & kWantW, want & kWantB, rows, cin, cout);
     if (!want) return SA_OK;
@@ -540,15 +574,17 @@ extern "C" int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int
     Scratch s{nullptr};
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{nullptr, cin, rows, cin, (flags & 1) != 0},
                   Matrix{nullptr, cout, cin, cout, (flags & 2) != 0}, Matrix{nullptr, cout, rows, cout, (flags & 4) != 0},
-                  Matrix{nullptr, cout, rows, cout, true}, act, want);
+                  Matrix{nullptr, cout, rows, cout, true}, act, two, want);
     *bytes = s.used;
     return SA_OK;
 }
 
 extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,
-                                 const void *g, long ldg, const void *z, long ldz, int act, void *dx, void *dw, void *db,
+                                 const void *g, long ldg, const void *z, long ldz, int activation, void *dx, void *dw, void *db,
                                  int db_f32, void *ws, unsigned long ws_bytes, void *stream) {
-    if (!sizes_ok(dtype, rows, cin, cout) || act < kNone || act > kSilu) return SA_ERR_INVALID;
+    int act;
+    bool two;
+    if (!sizes_ok(dtype, rows, cin, cout) || !take_act(dtype, activation, act, two)) return SA_ERR_INVALID;
     const int want = wanted(dx, dw, db, rows, cin, cout);
     if (!want) return SA_OK;
     if (rows && cout && (!g || ldg < cout || (act != kNone && (!z || ldz < cout)))) return SA_ERR_INVALID;
@@ -562,7 +598,7 @@ extern "C" int sa_dense_backward(int dtype, long rows, int cin, int cout, const 
     Scratch s{(char *)ws};
     plan_backward(b, s, dtype, rows, cin, cout, Matrix{x, ldx, rows, cin, aligned(x, ldx, dtype)},
                   Matrix{w, ldw, cin, cout, aligned(w, ldw, dtype)}, Matrix{g, ldg, rows, cout, aligned(g, ldg, dtype)},
-                  Matrix{z, ldz, rows, cout, aligned(z, ldz, dtype)}, act, want);
+                  Matrix{z, ldz, rows, cout, aligned(z, ldz, dtype)}, act, two, want);
     if (!scratch_ok(ws, s.used, ws_bytes)) return SA_ERR_INVALID;
     hipStream_t st = (hipStream_t)stream;
     int rc = launch_jobs(dtype, b.jobs, b.njobs, st);

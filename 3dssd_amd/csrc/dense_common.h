@@ -14,7 +14,8 @@
 namespace dense {
 
 enum Type { kF32 = 0, kBF16 = 1, kF16 = 2 };
-enum Act { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4 };
+enum Act { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4, kPlanes = 5 };      // kPlanes: see Product::zact
+constexpr int kRoundSlopes = 16;      // added to a gradient's activation: a 16-bit dZ is rounded instead of going in two planes
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -111,6 +112,28 @@ __device__ __forceinline__ float times_slope(float g, float z) {
         return g * (fabsf(z) > 110.0f ? s : s + z * s * (1.0f - s));
     }
     return g;
+}
+
+// dZ = G act'(Z) as an operand of 16-bit matrix instructions.  One rounding of it to the layer's type would add its own half step to
+// that of each result (an error 1.4 times as large), so it goes in two planes: what truncation leaves, and the rest, rounded -- to
+// 2^-16 of a bf16 dZ, 2^-22 of a fp16 one.  fp16's second plane is 2048 times the rest, or dZ below 2^-13 would have none (so it
+// reaches down to 2^-35).  Truncated, both planes have one sign, and neither is 0 unless dZ or its first plane is (an exact dZ's
+// second plane is the smallest number): an infinite weight gives an infinity, not NaN.  ReLU's dZ is G itself or 0: one plane.
+template <class T> struct Low;
+template <> struct Low<bf16_t> { static constexpr float scale = 1.0f; static constexpr int inf = 0x7f80; };
+template <> struct Low<f16_t> { static constexpr float scale = 2048.0f; static constexpr int inf = 0x7c00; };
+template <class T> __device__ __forceinline__ T truncated(float v);
+template <> __device__ __forceinline__ bf16_t truncated<bf16_t>(float v) { return bf16_t{(unsigned short)(__float_as_uint(v) >> 16)}; }
+template <> __device__ __forceinline__ f16_t truncated<f16_t>(float v) {
+    return f16_t{(unsigned short)__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(v, 0.0f))};
+}
+template <class T>
+__device__ __forceinline__ void split_slope(float d, T &high, T &low) {
+    high = truncated<T>(d);
+    unsigned short l = from_f32<T>((d - to_f32<T>(high)) * Low<T>::scale).u;
+    // nothing left, or infinity less itself
+    if ((unsigned short)((l & 0x7fff) - 1) >= Low<T>::inf) l = high.u & 0x7fff ? (high.u & 0x8000) | 1 : 0;
+    low.u = l;
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------
@@ -212,7 +235,7 @@ struct Product {
     int vec_a, vec_b;     // 16-byte aligned base and rows
     int splits;           // the k range is cut into this many pieces, each summed by a workgroup of its own
     long kchunk;          // k indices (tiles: steps) of one piece
-    int passes;           // tiles: 1, or 6 for fp32 operands in three bf16 planes each
+    int passes;           // tiles: 1; 6 for fp32 operands in three bf16 planes each; 2 for a dZ in two (the second plane first)
     long plane_a, plane_b;   // elements between planes
     float *part;          // splits > 1: [splits][M][Np] partial sums, Np = N rounded up to a multiple of 4
     Epilogue e;
@@ -221,7 +244,9 @@ struct Product {
     // small backward products
     const void *z;        // operand G becomes G act'(z), or null
     long ldz;
-    int vec_z, zact;
+    int vec_z;
+    int zact;             // the activation; kPlanes: G and z are the two planes of dZ
+    int two;              // 16-bit types: dZ in two planes, formed or read
     void *colsum;         // dW: sums of B over k, or null
     int col_f32;
     float *colpart;       // splits > 1: [splits][N]

@@ -157,6 +157,15 @@ template <class T, int N> struct Operand {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[t][j] = (short)from_f32<T>(v[j]).u;
     }
+    __device__ __forceinline__ void set(int t, const float *v, Operand &low) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            T high, rest;
+            split_slope<T>(v[j], high, rest);
+            f[t][j] = (short)high.u;
+            low.f[t][j] = (short)rest.u;
+        }
+    }
 };
 template <int N> struct Operand<float, N> {
     float f[N][8];
@@ -177,10 +186,17 @@ __device__ __forceinline__ void take(Operand<T, N> &o, const typename Side<T, RO
         }
     }
 }
-// dZ = G act'(Z) in place of G, rounded to the type as an operand of the products; sums += the unrounded values, if wanted
-template <class T, bool ROWS, int N>
-__device__ __forceinline__ void take_slope(Operand<T, N> &o, const typename Side<T, ROWS, N>::Regs &g,
+// dZ = G act'(Z) in place of G, as an operand of the products: in 16-bit types in two planes (LOW; or g and z are those planes
+// already) or rounded; sums += the values as they were, if wanted
+template <class T, bool ROWS, int N, bool LOW>
+__device__ __forceinline__ void take_slope(Operand<T, N> &o, Operand<T, N> &low, const typename Side<T, ROWS, N>::Regs &g,
                                            const typename Side<T, ROWS, N>::Regs &z, int act, bool summed, float *sums) {
+    if constexpr (LOW)
+        if (act == kPlanes) {
+            take<T, ROWS, N>(o, g);
+            take<T, ROWS, N>(low, z);
+            return;
+        }
 #pragma unroll
     for (int t = 0; t < N; ++t) {
         float d[8];
@@ -189,7 +205,8 @@ __device__ __forceinline__ void take_slope(Operand<T, N> &o, const typename Side
             for (int j = 0; j < 8; ++j)
                 d[j] = times_slope<decltype(a)::value>(Side<T, ROWS, N>::at(g, t, j), Side<T, ROWS, N>::at(z, t, j));
         });
-        o.set(t, d);
+        if constexpr (LOW) o.set(t, d, low);
+        else o.set(t, d);
         if (summed)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sums[t] += d[j];
@@ -241,13 +258,13 @@ __device__ __forceinline__ void meet() {
 
 // Block `pos` of a product, k piece `piece`, by NW neighbouring waves, with `sums` for them alone; the workgroup's other waves do
 // the same with blocks of their own, or beyond the last.  Z: A (ZSIDE 0) or B (ZSIDE 1) is G, and the product takes
-// G act'(Z) with Z = P.z in G's place (rows of P.ldz).
-template <class T, bool TA, bool TB, int NA, int NB, int NW, int ZSIDE>
+// G act'(Z) with Z = P.z in G's place (rows of P.ldz), with LOW in two planes.
+template <class T, bool TA, bool TB, int NA, int NB, int NW, int ZSIDE, bool LOW = false>
 __device__ __forceinline__ void block_product(const Product &P, unsigned pos, int piece, float *sums) {
     constexpr int E = sizeof(T), kM = 16 * NA, kN = 16 * NB;
     // steps in flight, by the registers of one; four waves of a 32 x 32 block have one step each
     constexpr int kSlot = 2 * E * (NA + NB + (ZSIDE == 0 ? NA : ZSIDE == 1 ? NB : 0));
-    constexpr int kAhead = few_steps(NA, NB, NW) ? 1 : kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
+    constexpr int kAhead = few_steps(NA, NB, NW) || LOW ? 1 : kSlot <= 16 ? 4 : kSlot <= 32 ? 2 : 1;
     static_assert(NW * kM * kN <= kSums, "the waves' sums");
     const int thread = threadIdx.x % (NW * 64), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const unsigned nb = (unsigned)((P.N + kN - 1) / kN);
@@ -272,6 +289,8 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
     if (ZSIDE >= 0) z.init(lane, P.ldz, (ZSIDE == 1 ? P.N : P.M) - z0);
 
     f4 acc[NB][NA] = {};
+    constexpr bool kApart = LOW && __is_same(T, f16_t);        // fp16's second plane has a scale
+    f4 apart[kApart ? NB : 1][kApart ? NA : 1] = {};
     float column[NB] = {};                             // sums of B's rows over k (the bias gradient), where wanted
     const bool summed = P.colsum && m0 == 0;
     typename SA::Regs ra[kAhead];
@@ -286,12 +305,12 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
         if constexpr (ZSIDE >= 0) z.fetch(rz[slot], Z + s * stepz, left, P.vec_z);
     };
     auto products = [&](int slot) {
-        Operand<T, NA> oa;
-        Operand<T, NB> ob;
-        if constexpr (ZSIDE == 0) take_slope<T, TA, NA>(oa, ra[slot], rz[slot], P.zact, false, nullptr);
+        Operand<T, NA> oa, la;
+        Operand<T, NB> ob, lb;
+        if constexpr (ZSIDE == 0) take_slope<T, TA, NA, LOW>(oa, la, ra[slot], rz[slot], P.zact, false, nullptr);
         else take<T, TA, NA>(oa, ra[slot]);
         if constexpr (ZSIDE == 1) {
-            take_slope<T, TB, NB>(ob, rb[slot], rz[slot], P.zact, summed, column);
+            take_slope<T, TB, NB, LOW>(ob, lb, rb[slot], rz[slot], P.zact, summed, column);
         } else {
             take<T, TB, NB>(ob, rb[slot]);
             if (summed)
@@ -299,6 +318,12 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
                 for (int t = 0; t < NB; ++t)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) column[t] += SB::at(rb[slot], t, j);
+        }
+        if constexpr (LOW) {
+            const Operand<T, NA> &xa = ZSIDE == 0 ? la : oa;
+            const Operand<T, NB> &xb = ZSIDE == 1 ? lb : ob;
+            if constexpr (kApart) multiply<T, NA, NB>(apart, xa, xb);
+            else multiply<T, NA, NB>(acc, xa, xb);
         }
         multiply<T, NA, NB>(acc, oa, ob);
     };
@@ -314,6 +339,11 @@ __device__ __forceinline__ void block_product(const Product &P, unsigned pos, in
         }
     }
 
+    if constexpr (kApart)
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+            for (int y = 0; y < NB; ++y) acc[y][x] += apart[y][x] * (1.0f / Low<T>::scale);
 #pragma unroll
     for (int x = 0; x < NA; ++x)
 #pragma unroll
@@ -375,28 +405,28 @@ __global__ __launch_bounds__(NW * 64, few_steps(NA, NB, NW) ? 5 : NW / 4) void s
 }
 
 // A workgroup's share of a product: block `group`, or with P.alone (ALONE: which may be set) a block for each of its waves.
-template <class T, bool TA, bool TB, int WT, int NW, int ZSIDE, bool ALONE>
+template <class T, bool TA, bool TB, int WT, int NW, int ZSIDE, bool ALONE, bool LOW = false>
 __device__ __forceinline__ void group_product(const Product &P, unsigned group, int piece, float *sums) {
     if (!ALONE || !P.alone) {
-        block_product<T, TA, TB, WT, WT, NW, ZSIDE>(P, group, piece, sums);
+        block_product<T, TA, TB, WT, WT, NW, ZSIDE, LOW>(P, group, piece, sums);
     } else {
         const unsigned mine = threadIdx.x >> 6;
-        block_product<T, TA, TB, WT, WT, 1, ZSIDE>(P, group * NW + mine, piece, sums + mine * (256 * WT * WT));
+        block_product<T, TA, TB, WT, WT, 1, ZSIDE, LOW>(P, group * NW + mine, piece, sums + mine * (256 * WT * WT));
     }
 }
 
 // dX and dW of a layer in one launch: the workgroups from x0 to x1 are dX's (all blocks of a piece, then the next piece), the
 // others, in front of those or behind, dW's.  dW's blocks have WT x WT MFMA tiles.  128 registers: two workgroups of eight
-// waves per CU.
-template <class T, bool Z, int WT, int NW, bool ALONE>
+// waves per CU.  Z: 0 without slopes, 1 with, 2 with, in two planes.
+template <class T, int Z, int WT, int NW, bool ALONE>
 __global__ __launch_bounds__(NW * 64, 4) void small_backward_kernel(Product X, Product W, unsigned x0, unsigned x1) {
     __shared__ __attribute__((aligned(16))) float sums[NW * 1024];
     if (blockIdx.x < x0 || blockIdx.x >= x1) {
         const unsigned b = blockIdx.x < x0 ? blockIdx.x : blockIdx.x - x1, groups = (gridDim.x - (x1 - x0)) / W.splits;
-        group_product<T, true, true, WT, NW, Z ? 1 : -1, ALONE>(W, W.first + on_xcd(b % groups, groups), b / groups, sums);
+        group_product<T, true, true, WT, NW, Z ? 1 : -1, ALONE, Z == 2>(W, W.first + on_xcd(b % groups, groups), b / groups, sums);
     } else {
         const unsigned b = blockIdx.x - x0, groups = (x1 - x0) / X.splits;
-        group_product<T, false, false, 2, NW, Z ? 0 : -1, ALONE>(X, X.first + on_xcd(b % groups, groups), b / groups, sums);
+        group_product<T, false, false, 2, NW, Z ? 0 : -1, ALONE, Z == 2>(X, X.first + on_xcd(b % groups, groups), b / groups, sums);
     }
 }
 
@@ -468,7 +498,7 @@ int launch_forward(Product P, hipStream_t s) {
 }
 
 // nx, nw: blocks of a piece
-template <class T, bool Z, int WT, int NW>
+template <class T, int Z, int WT, int NW>
 int launch_backward(Product X, Product W, long nx, long nw, hipStream_t s) {
     // One wave's steps are few where a layer is narrow on one side, and the product on that side all output: fp32 6 x 3217 x
     // 16023, whose dW is 200 MB of sums of six terms, takes 190 us instead of 412.  (With a few workgroups only, the waves
@@ -498,7 +528,7 @@ int launch_backward(Product X, Product W, long nx, long nw, hipStream_t s) {
     });
 }
 template <class T, int WT>
-int launch_backward(const Product &X, Product W, long nx, bool z, hipStream_t s) {
+int launch_backward(const Product &X, Product W, long nx, hipStream_t s) {
     constexpr long E = sizeof(T);
     long nw = 0;
     if (W.a || W.colsum || W.e.y) {
@@ -508,8 +538,10 @@ int launch_backward(const Product &X, Product W, long nx, bool z, hipStream_t s)
         nw = blocks_of(W, 16 * WT, 16 * WT);
     }
     const bool shorter = (nx == 0 || X.kchunk <= 128) && (nw == 0 || W.kchunk <= 128);
-    if (z) return shorter ? launch_backward<T, true, WT, 4>(X, W, nx, nw, s) : launch_backward<T, true, WT, 8>(X, W, nx, nw, s);
-    return shorter ? launch_backward<T, false, WT, 4>(X, W, nx, nw, s) : launch_backward<T, false, WT, 8>(X, W, nx, nw, s);
+    if constexpr (E == 2)
+        if (X.two || W.two) return shorter ? launch_backward<T, 2, WT, 4>(X, W, nx, nw, s) : launch_backward<T, 2, WT, 8>(X, W, nx, nw, s);
+    if (X.z || W.z) return shorter ? launch_backward<T, 1, WT, 4>(X, W, nx, nw, s) : launch_backward<T, 1, WT, 8>(X, W, nx, nw, s);
+    return shorter ? launch_backward<T, 0, WT, 4>(X, W, nx, nw, s) : launch_backward<T, 0, WT, 8>(X, W, nx, nw, s);
 }
 template <class T>
 int launch_backward(const Product *px, const Product *pw, hipStream_t s) {
@@ -518,11 +550,10 @@ int launch_backward(const Product *px, const Product *pw, hipStream_t s) {
     if (px) X = *px;
     if (pw) W = *pw;
     const long nx = px ? blocks_of(X, 32, 32) : 0;
-    const bool z = X.z || W.z;
     // fp32 products take a CU long (16 x 16 x 4 per MFMA of 32 cycles): smaller blocks where there are few
     if constexpr (sizeof(T) == 4)
-        if (blocks_of(W, 32, 32) * W.splits < 256) return launch_backward<T, 1>(X, W, nx, z, s);
-    return launch_backward<T, 2>(X, W, nx, z, s);
+        if (blocks_of(W, 32, 32) * W.splits < 256) return launch_backward<T, 1>(X, W, nx, s);
+    return launch_backward<T, 2>(X, W, nx, s);
 }
 
 }  // namespace

@@ -33,9 +33,12 @@ constexpr int kBK = 64;
 
 // Planes of a fp32 operand (dense.hip): which plane of A meets which of B, the smallest terms first
 __device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1, 0, 1, 0};
+// Of two passes the first has the second plane of dZ; the other operand has one plane (and 0 elements to the next)
+__device__ __forceinline__ int plane_of(const int (&table)[6], int pass, int passes) { return passes == 2 ? 1 - pass : table[pass]; }
 
 template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB>
 __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
+    constexpr bool kCarries = __is_same(MT, f16_t) && TA == TB;        // (a gradient's product)
     constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, kA = BM * kBK * 2, kB = BN * kBK * 2;
     static_assert(FN == 4 && kA == W * 4096, "the epilogue takes 16 x 64 of a wave at a time, in the wave's share of a buffer");
     __shared__ __attribute__((aligned(1024))) char lds[3 * kA + 2 * kB];
@@ -73,8 +76,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
     auto start_pass = [&]() {                              // a rare one: the product's description is read again
         const Product &R = arguments();
         const Place p = place<BM, BN, kBK>(R, load_item - stride);
-        at_a = (const char *)R.a + ((TA ? p.m0 : p.m0 * R.lda) + (R.passes > 1 ? kPlaneA[pass] * R.plane_a : 0)) * 2 + (long)kstep * step_a;
-        at_b = (const char *)R.b + ((TB ? p.n0 : p.n0 * R.ldb) + (R.passes > 1 ? kPlaneB[pass] * R.plane_b : 0)) * 2 + (long)kstep * step_b;
+        at_a = (const char *)R.a + ((TA ? p.m0 : p.m0 * R.lda) + (R.passes > 1 ? plane_of(kPlaneA, pass, R.passes) * R.plane_a : 0)) * 2 + (long)kstep * step_a;
+        at_b = (const char *)R.b + ((TB ? p.n0 : p.n0 * R.ldb) + (R.passes > 1 ? plane_of(kPlaneB, pass, R.passes) * R.plane_b : 0)) * 2 + (long)kstep * step_b;
     };
     auto next = [&]() {
         if (load_left == 0 && load_item < end) {
@@ -154,24 +157,40 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
     __builtin_amdgcn_s_barrier();
     unsigned a0 = base, b0 = base + 3 * kA;            // this step's buffers
     for (; item < end; item += stride) {
-        const int steps = place<BM, BN, kBK>(arguments(), item).steps;
-        // (the last half before read these too; kept from there they would take 48 registers through the end of the tile)
-#pragma unroll
-        for (int op = 0; op < FM + FN; ++op) read(f0, a0, b0, 0, op);
+        const Place whole = place<BM, BN, kBK>(arguments(), item);
+        // fp16's second plane of dZ has a scale: what its pass, the first of two, has summed loses it before the next
+        int run = whole.steps, rest = 0;
+        if constexpr (kCarries)
+            if (arguments().passes == 2) {
+                run = per - whole.first < 0 ? 0 : per - whole.first < run ? per - whole.first : run;
+                rest = whole.steps - run;
+            }
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int i = 0; i < FM; ++i) acc[j][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int step = 0; step < steps; ++step) {
-            next();
-            half(f0, f1, a0, b0, 1, load_a, LA);
-            // step + 1 has arrived (this wave's part; the barrier makes it everyone's), and everyone has read all of this one
-            __builtin_amdgcn_s_waitcnt(wait_code(LA));
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            a0 = a0 == base + 2 * kA ? base : a0 + kA;
-            b0 = base + 3 * kA + kB - (b0 - base - 3 * kA);
-            half(f1, f0, a0, b0, 0, load_b, LB);
+#pragma unroll 1
+        for (int part = 0;; ++part) {
+            // (the last half before read these too; kept from there they would take 48 registers through the end of the tile)
+#pragma unroll
+            for (int op = 0; op < FM + FN; ++op) read(f0, a0, b0, 0, op);
+            for (int step = 0; step < run; ++step) {
+                next();
+                half(f0, f1, a0, b0, 1, load_a, LA);
+                // step + 1 has arrived (this wave's part; the barrier makes it everyone's), and everyone has read all of this one
+                __builtin_amdgcn_s_waitcnt(wait_code(LA));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                a0 = a0 == base + 2 * kA ? base : a0 + kA;
+                b0 = base + 3 * kA + kB - (b0 - base - 3 * kA);
+                half(f1, f0, a0, b0, 0, load_b, LB);
+            }
+            if (!kCarries || part == 1 || arguments().passes != 2) break;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[j][i] *= 1.0f / Low<f16_t>::scale;
+            run = rest;
         }
 
         leave_tile<BM, BN, kBK, W, OT>(acc, item, wm, wn, wave, lane, to_a);

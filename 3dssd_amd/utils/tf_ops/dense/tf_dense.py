@@ -23,6 +23,7 @@ from ... import _native as N
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_ROUND_SLOPES = 16                    # added to the activation's number
 _FAR = 1 << 24                        # rows further apart than this are copied together; longer ones are refused
 
 
@@ -132,16 +133,16 @@ def dense(inputs, weights, biases=None, activation=None, residual=None, return_p
     return (out, pre) if return_preact else out
 
 
-def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=None, needs=(True, True), round_slopes=True):
+def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=None, needs=(True, True), round_slopes=False):
     """Gradient of dense: (grad_inputs [..., cin], grad_weights [cin, cout], grad_biases [cout]).
 
     grad_out [..., cout] is the gradient of dense's out (and, unchanged, the gradient of its residual); preact is the z that
     dense(..., return_preact=True) returned, needed with an activation.  ReLU's slope at 0 is 0.  needs: whether the first
     two are wanted (None in their place if not); grad_biases is computed where biases are given and has their type.
-    With an activation the 16-bit forms round grad_out * slope once to the inputs' type, as an operand of both products; the
-    bias gradient sums it unrounded.  The results' relative error (2-norm) is then 1.4 times what rounding them alone makes.
-    round_slopes=False keeps that product in 32 bits: the layer is taken through the fp32 kernels, at three to five times the
-    time and with copies of the operands in fp32 (8192 x 4096 x 8192 bf16: 0.89 ms and an error of 2.3e-3, or 4.6 ms and 1.7e-3).
+    With GELU or SiLU the 16-bit forms take grad_out * slope into both products in two planes of the type (to 2^-16 of itself in
+    bf16, 2^-22 or 2^-35 in fp16), which is twice the products of the forward pass each.  round_slopes=True rounds it once to
+    the type instead: up to half the time, and results with 1.4 times the relative error (2-norm) that rounding them alone
+    makes.  The bias gradient sums it unrounded either way.
     Sums run in fp32 in a fixed order: the same call gives the same bits."""
     dt, cin, cout = _layer("DenseGrad", inputs, weights, biases, activation)
     shape = inputs.shape[:-1] + (cout,)
@@ -154,10 +155,6 @@ def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=N
         _beside(preact, "preact", inputs)
         T.require(preact.shape == shape, "DenseGrad expects (...,cout) preact shape")
     T.require(len(needs) == 2, "needs: (inputs, weights)")
-    if not round_slopes and activation is not None and dt != torch.float32:
-        wide = dense_grad(inputs.float(), weights.float(), grad_out.float(), None if biases is None else biases.float(),
-                          activation, preact.float(), needs)
-        return tuple(None if t is None else t.to(to) for t, to in zip(wide, (dt, dt, biases.dtype if biases is not None else dt)))
     dx = inputs.new_empty(inputs.shape) if needs[0] else None
     dw = inputs.new_empty((cin, cout)) if needs[1] else None
     db = biases.new_empty((cout,)) if biases is not None else None
@@ -168,7 +165,7 @@ def dense_grad(inputs, weights, grad_out, biases=None, activation=None, preact=N
     w, wp, ldw = _rows(weights, cout) if cin and cout else (None, None, cout)
     g, gp, ldg = _rows(grad_out, cout) if rows and cout else (None, None, cout)
     z, zp, ldz = _rows(preact, cout) if preact is not None and rows and cout else (None, None, cout)
-    code, e, act = TYPES[dt], dt.itemsize, ACTIVATIONS[activation]
+    code, e, act = TYPES[dt], dt.itemsize, ACTIVATIONS[activation] + (_ROUND_SLOPES if round_slopes else 0)
     want = ((1 if dx is not None and rows and cin else 0) | (2 if dw is not None and cin and cout else 0)
             | (4 if db is not None and cout else 0))
     if want:

@@ -266,7 +266,8 @@ int sa_dense_forward(int dtype, long rows, int cin, int cout, const void *x, lon
                      unsigned long ws_bytes, sa_stream_t stream);
 /* Gradient: dz = g act'(z), dx = dz W^T [rows,cin], dw = x^T dz [cin,cout], db = column sums of dz [cout] (fp32 where
  * db_f32), each nullable and dense; g, z [rows,cout] (ldg, ldz; z = pre of the forward call, unused with act 0).  16-bit
- * types round dz once, as an operand of the products.  want (of the _ws call): bit 0 / 1 / 2 = dx / dw / db; flags: bit
+ * types with act 2 to 4 take dz into the products in two planes (bf16: to 2^-16 of itself; fp16: to 2^-22 of itself or 2^-35,
+ * whichever is larger), or, with 16 added to act, rounded once to the type, at half the time.  want (of the _ws call): bit 0 / 1 / 2 = dx / dw / db; flags: bit
  * 0 / 1 / 2 = x / W / g is aligned as above. */
 int sa_dense_backward_ws(int dtype, long rows, int cin, int cout, int act, int want, int flags, unsigned long *bytes);
 int sa_dense_backward(int dtype, long rows, int cin, int cout, const void *x, long ldx, const void *w, long ldw,

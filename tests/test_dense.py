@@ -535,32 +535,99 @@ def test_a_training_step_of_a_residual_block(gpu, dt):
         close(got, want * (5.0 / ref), what)
 
 
+def _held(d, dt):
+    """How far the two planes of a 16-bit dz may be from it.  bf16: truncated to 8 bits, a step of 2^-7 of its power of two is left, of
+    which 8 bits are rounded: 2^-16.  fp16: 11 and 11 bits, 2^-22, and the second plane's smallest number over 2048, 2^-35."""
+    return {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}[dt] * d.abs() + 2.0 ** -35 * (dt == torch.float16)
+
+
+def _check_unrounded(x, w, g, act, z, dx, dw, db):
+    """As _check_grad, with a dz that is not rounded to the type."""
+    gd = g.double()
+    d = gd * _slope64(z.double(), act)
+    dd = 0 * d if act is None else 32 * U * gd.abs() * (1 + z.double().abs()) + _tiny(torch.float32)
+    dr = dd if act in (None, "relu") else dd + _held(d, x.dtype)
+    wt, xt = w.double().t().contiguous(), x.double().t().contiguous()
+    for got, want, bound, what in (
+            (dx, lambda: d @ wt, lambda: (_sum_bound(w.shape[1]) * (d.abs() + dr) + dr) @ wt.abs(), "grad_inputs"),
+            (dw, lambda: xt @ d, lambda: xt.abs() @ (_sum_bound(x.shape[0]) * (d.abs() + dr) + dr), "grad_weights"),
+            (db, lambda: d.sum(0), lambda: (_sum_bound(x.shape[0]) * (d.abs() + dd) + dd).sum(0), "grad_biases")):
+        if got is not None:
+            want, bound = want(), bound()
+            _within(got, want, _half(got.dtype) * (want.abs() + bound) + bound + _tiny(got.dtype), what)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("size", [(1, 64, 8), (129, 257, 130), (2048, 512, 128), (1100, 1100, 1100), (5003, 771, 1283)])
-def test_slopes_kept_in_32_bits(gpu, dt, size):
-    """round_slopes=False: no rounding of grad_out * slope, so what is left are the fp32 sums and one rounding per result."""
+@pytest.mark.parametrize("size", SIZES)
+def test_slopes_are_not_rounded(gpu, dt, size):
+    """What is left are the fp32 sums and one rounding per result."""
     m = _mod()
     rows, cin, cout = size
-    for i, act in enumerate(ACTS):
+    i = SIZES.index(size)
+    for act in (ACTS[2 + i % 3], ACTS[i % 2]):
         x, w = _rand(gpu, (rows, cin), dt, i), _rand(gpu, (cin, cout), dt, 10 + i, math.sqrt(2.0 / cin))
         g, z = _rand(gpu, (rows, cout), dt, 20 + i, 0.05), _rand(gpu, (rows, cout), dt, 30 + i)
         b = torch.empty(cout, dtype=(dt, torch.float32)[i % 2], device=gpu)
-        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z, round_slopes=False)
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z)
         assert dx.dtype == dw.dtype == dt and db.dtype == b.dtype
-        d = g.double() * _slope64(z.double(), act)
-        dd = 0 * d if act is None else 32 * U * g.double().abs() * (1 + z.double().abs()) + _tiny(torch.float32)
-        wt, xt = w.double().t().contiguous(), x.double().t().contiguous()
-        for got, want, bound, what in (
-                (dx, d @ wt, (_sum_bound(cout) * (d.abs() + dd) + dd) @ wt.abs(), "grad_inputs"),
-                (dw, xt @ d, xt.abs() @ (_sum_bound(rows) * (d.abs() + dd) + dd), "grad_weights"),
-                (db, d.sum(0), (_sum_bound(rows) * (d.abs() + dd) + dd).sum(0), "grad_biases")):
-            _within(got, want, _half(got.dtype) * (want.abs() + bound) + bound + _tiny(got.dtype), what)
-        only = m.dense_grad(x, w, g, activation=act, preact=z, needs=(False, True), round_slopes=False)
+        _check_unrounded(x, w, g, act, z, dx, dw, db)
+        only = m.dense_grad(x, w, g, activation=act, preact=z, needs=(False, True))
         assert only[0] is None and torch.equal(only[1], dw) and only[2] is None
-        if dt == torch.float32 or act is None:         # nothing is rounded there either way
-            for a, b_ in zip((dx, dw, db), m.dense_grad(x, w, g, biases=b, activation=act, preact=z)):
-                assert torch.equal(a, b_)
+        only = m.dense_grad(x, w, g, activation=act, preact=z, needs=(True, False))
+        assert only[1] is None and torch.equal(only[0], dx) and only[2] is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_slopes_rounded_where_the_caller_says_so(gpu, dt, size):
+    m = _mod()
+    rows, cin, cout = size
+    i = SIZES.index(size)
+    act = ACTS[(i + 3) % 5]
+    x, w = _rand(gpu, (rows, cin), dt, i), _rand(gpu, (cin, cout), dt, 10 + i, math.sqrt(2.0 / cin))
+    g, z = _rand(gpu, (rows, cout), dt, 20 + i, 0.05), _rand(gpu, (rows, cout), dt, 30 + i)
+    b = torch.empty(cout, dtype=(dt, torch.float32)[i % 2], device=gpu)
+    dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z, round_slopes=True)
+    _check_grad(x, w, g, act, z, dx, dw, db)
+    for needs in ((True, False), (False, True)):
+        only = m.dense_grad(x, w, g, activation=act, preact=z, needs=needs, round_slopes=True)
+        assert all(a is None or torch.equal(a, b_) for a, b_ in zip(only, (dx, dw, db)))
+    if dt == torch.float32 or act in (None, "relu"):   # nothing is rounded there either way
+        for a, b_ in zip((dx, dw, db), m.dense_grad(x, w, g, biases=b, activation=act, preact=z)):
+            assert torch.equal(a, b_)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("size", [(3, 64, 40), (300, 100, 260), (4, 64, 1100), (600, 500, 400), (1100, 1100, 1100), (1200, 1104, 1112)])
+def test_small_slopes_and_infinite_factors(gpu, size, dt):
+    """Gradients near the end of fp16's range keep their bits in the sums over many rows.  Infinite inputs, weights and gradients give
+    the infinities of the product's sign and NaN where an infinity meets 0 or its opposite."""
+    m = _mod()
+    rows, cin, cout = size
+    inf = float("inf")
+    for act in ACTS[2:]:
+        x, w = _rand(gpu, (rows, cin), dt, 1), _rand(gpu, (cin, cout), dt, 2)
+        g, z = _rand(gpu, (rows, cout), dt, 3, 2e-6), _rand(gpu, (rows, cout), dt, 4, 2.0)
+        b = torch.empty(cout, dtype=torch.float32, device=gpu)
+        _check_unrounded(x, w, g, act, z, *m.dense_grad(x, w, g, biases=b, activation=act, preact=z))
+        # now dz of a size that the first plane has, and no exact one
+        g, z = _rand(gpu, (rows, cout), dt, 5), _rand(gpu, (rows, cout), dt, 6).clamp(-0.6, 0.6)
+        g = torch.where(g.abs() < 1e-2, torch.ones((), dtype=dt, device=gpu), g)
+        z[0, :3], g[0, :3] = 0.0, 1.0                  # and some exact ones: slope 1 / 2
+        w[5, 7], w[7, 7], x[1, 3], x[rows - 1, 5] = inf, -inf, inf, -inf
+        w[9, 2] = 0.0
+        g[2, 4], g[2, 2] = inf, -inf
+        dx, dw, db = m.dense_grad(x, w, g, biases=b, activation=act, preact=z)
+        d = g.double() * _slope64(z.double(), act)
+        big = torch.finfo(dt).max
+        for got, want in ((dx, d @ w.double().t().contiguous()), (dw, x.double().t().contiguous() @ d), (db, d.sum(0))):
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            for s in (1, -1):
+                assert torch.equal(got == s * inf, want == s * inf)
+            assert float(want[torch.isfinite(want)].abs().max()) < big / 2
 
 
 @pytest.mark.gpu
