@@ -36,9 +36,10 @@ __device__ constexpr int kPlaneA[6] = {2, 0, 1, 1, 0, 0}, kPlaneB[6] = {0, 2, 1,
 // Of two passes the first has the second plane of dZ; the other operand has one plane (and 0 elements to the next)
 __device__ __forceinline__ int plane_of(const int (&table)[6], int pass, int passes) { return passes == 2 ? 1 - pass : table[pass]; }
 
-template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB>
+// CARRY: two passes of fp16, of which the first's operand has a scale.  (In a kernel of its own: the tile's end spills for it, and one
+// pass of 4096^3 took 250 us in both gradients instead of 235.)
+template <int BM, int BN, int WM, int WN, class MT, class OT, bool TA, bool TB, bool CARRY = false>
 __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
-    constexpr bool kCarries = __is_same(MT, f16_t) && TA == TB;        // (a gradient's product)
     constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, kA = BM * kBK * 2, kB = BN * kBK * 2;
     static_assert(FN == 4 && kA == W * 4096, "the epilogue takes 16 x 64 of a wave at a time, in the wave's share of a buffer");
     __shared__ __attribute__((aligned(1024))) char lds[3 * kA + 2 * kB];
@@ -160,11 +161,10 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
         const Place whole = place<BM, BN, kBK>(arguments(), item);
         // fp16's second plane of dZ has a scale: what its pass, the first of two, has summed loses it before the next
         int run = whole.steps, rest = 0;
-        if constexpr (kCarries)
-            if (arguments().passes == 2) {
-                run = per - whole.first < 0 ? 0 : per - whole.first < run ? per - whole.first : run;
-                rest = whole.steps - run;
-            }
+        if constexpr (CARRY) {
+            run = per - whole.first < 0 ? 0 : per - whole.first < run ? per - whole.first : run;
+            rest = whole.steps - run;
+        }
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_kernel(Product P) {
                 b0 = base + 3 * kA + kB - (b0 - base - 3 * kA);
                 half(f1, f0, a0, b0, 0, load_b, LB);
             }
-            if (!kCarries || part == 1 || arguments().passes != 2) break;
+            if (!CARRY || part == 1) break;
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -203,9 +203,14 @@ int launch(bool ta, bool tb, const Product &P, int slots, hipStream_t s) {
     const long items = ((P.M + BM - 1) / BM) * ((P.N + BN - 1) / BN) * P.splits;
     if (items > 0x3fffffffL) return SA_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(items < slots ? items : slots)), block(WM * WN * 64);
-    if (ta) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, true, true>), grid, block, 0, s, P);
-    else if (tb) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, true>), grid, block, 0, s, P);
-    else hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, false>), grid, block, 0, s, P);
+    auto go = [&](auto carry) {
+        constexpr bool C = decltype(carry)::value;
+        if (ta) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, true, true, C>), grid, block, 0, s, P);
+        else if (tb) hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, true>), grid, block, 0, s, P);
+        else hipLaunchKernelGGL((tile_kernel<BM, BN, WM, WN, MT, OT, false, false, C>), grid, block, 0, s, P);
+    };
+    if (__is_same(MT, f16_t) && P.passes == 2) go(Tag<__is_same(MT, f16_t)>{});
+    else go(Tag<0>{});
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
