@@ -21,6 +21,6 @@ int launch_split(bool ta, const Product &P, hipStream_t s);
 // Any forward product (A k-contiguous, B n-contiguous); P.kchunk counts k indices (a multiple of 32).
 int launch_small_forward(int type, const Product &P, hipStream_t s);
 // dX (A = G or dZ and B = W, both k-contiguous) and dW (A = X, B = G or dZ, both with rows contiguous) in one launch; either
-// may be null.  With P.z set the operand G becomes G act'(Z); dW's colsum is the bias gradient.
+// may be null.  With P.z set the operand G becomes G act'(Z), with P.two in two planes; dW's colsum is the bias gradient.
 int launch_small_backward(int type, const Product *dx, const Product *dw, hipStream_t s);
 }  // namespace dense

@@ -5,8 +5,8 @@
 //
 // Against the tile kernel run six times over planes of both (dense_tile.hip): A is read once, as 4 bytes instead of six times
 // 2; no pass in front has to write 6 bytes for each of its values; and a fragment serves two or three products while it is in
-// registers, so LDS gives 36 KB per 32 k and wave instead of 72.  32768 x 1536 x 512: 227 us instead of 326 (fp32 matrix
-// instructions of a library: 362), 1.36 PFLOP/s of bf16 products, which is what large bf16 products reach on this chip.  With
+// registers, so LDS gives 36 KB per 32 k and wave instead of 72.  32768 x 1536 x 512: 223 us instead of 326 (fp32 matrix
+// instructions of a library: 362), 1.4 PFLOP/s of bf16 products, which is what large bf16 products reach on this chip.  With
 // little k to a tile, or few rows, the planes cost less than this kernel's single shape of tile: dense.hip compares.
 //
 // 256 x 256 tiles, eight waves of 128 x 64, steps of 32 k.  A wave holds B's twelve fragments of the step and walks over its
@@ -17,7 +17,7 @@
 //   block 7     reads the first fragments of the next step, each plane into the registers of one that is done with.
 // So each value is cut once per workgroup: with every wave cutting what it reads, four times as often, the same product took
 // 248 us.  One barrier after block 0 (B's LDS may be written), one after block 6 (the next step is complete).
-// Bound by the matrix instructions at the clock that their power leaves (2.0 GHz here, 68 % of the cycles busy).
+// Bound by the matrix instructions at the clock that their power leaves (2.0 GHz, 66 % of the cycles busy).
 #include "dense_common.h"
 #include "dense_lds.h"
 #include "dense_products.h"

@@ -12,7 +12,7 @@
 //                  launch read are still in the memory-side cache.  Out of place it copies even where nothing is clipped;
 //                  in place it then returns at once.  Lists beyond that cache are read and written past it (503 MB of
 //                  bf16: 280 -> 248 us); shorter ones stay in it for the optimizer that reads them next.
-// 503 MB: sums 88 us (5.7 TB/s), scaling 160 us (6.3 TB/s).  1024 workgroups: what the registers let reside at once (2048
+// 503 MB: sums 86 us (5.9 TB/s), scaling 161 us (6.2 TB/s).  1024 workgroups: what the registers let reside at once (2048
 // ran in two rounds, 115 us).
 // Longer lists: one launch of each kernel per 128 tensors, with norm_kernel between.
 // A norm that is not finite makes every output NaN, so that a step with such gradients cannot pass unseen.
